@@ -1118,10 +1118,14 @@ torch::Tensor tr_probe(int64_t scheme) {
 }
 
 }  // namespace
+
+void bind_encoder(pybind11::module& m);  // bindings_encoder.cpp
+
 }  // namespace colearn
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   using namespace colearn;
+  bind_encoder(m);
   m.def("fused_sgd", &fused_sgd);
   m.def("fused_adam", &fused_adam);
   m.def("sq_norm_per_row", &sq_norm_per_row);

@@ -1,0 +1,478 @@
+// Python bindings of the encoder-training kernels: masked attention, residual
+// add + layer norm, AdamW over many tensors.  Everything a kernel assumes of
+// its operands is checked here, before a launch.
+
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <limits>
+#include <optional>
+#include <utility>
+#include <vector>
+
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include "encoder_api.h"
+
+#define HIP_CHECK_LAST()                                          \
+  do {                                                            \
+    hipError_t e_ = hipGetLastError();                            \
+    TORCH_CHECK(e_ == hipSuccess, "HIP kernel launch failed: ",   \
+                hipGetErrorString(e_));                           \
+  } while (0)
+
+namespace colearn {
+
+namespace {
+
+using OptTensor = std::optional<torch::Tensor>;
+
+hipStream_t stream() {
+  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+}
+
+Elem elem_of(const torch::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32:
+      return Elem::kF32;
+    case torch::kBFloat16:
+      return Elem::kBF16;
+    case torch::kFloat16:
+      return Elem::kF16;
+    default:
+      TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, not ",
+                  t.scalar_type());
+  }
+}
+
+void check_gpu(const torch::Tensor& t, const torch::Device& dev,
+               const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == dev, name,
+              " must be on the GPU of the first operand (", dev, "), not ",
+              t.device());
+}
+
+void check_like(const torch::Tensor& t, const torch::Tensor& like,
+                const char* name) {
+  check_gpu(t, like.device(), name);
+  TORCH_CHECK(t.scalar_type() == like.scalar_type() &&
+                  t.sizes() == like.sizes(),
+              name, " must have the type and shape of the first operand");
+}
+
+bool aligned16(const torch::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// ---- AdamW ------------------------------------------------------------------
+void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
+                std::vector<torch::Tensor> m, std::vector<torch::Tensor> v,
+                std::vector<torch::Tensor> ms, std::vector<torch::Tensor> vs,
+                std::vector<torch::Tensor> ref, std::vector<double> keep,
+                double b1, double b2, double eps, double mu, double step,
+                double inv_bc2, OptTensor live) {
+  const size_t count = p.size();
+  if (count == 0) return;
+  const bool eight = !ms.empty(), prox = !ref.empty();
+  TORCH_CHECK(g.size() == count && m.size() == count && v.size() == count &&
+                  keep.size() == count && ms.size() == vs.size() &&
+                  (!eight || ms.size() == count) &&
+                  (!prox || ref.size() == count),
+              "adamw: the lists must have one entry a parameter");
+  const torch::Device dev = p[0].device();
+  TORCH_CHECK(dev.is_cuda(), "adamw: parameters must be on a GPU");
+  const auto pt = p[0].scalar_type(), gt = g[0].scalar_type();
+  auto real = [](torch::ScalarType t) {
+    return t == torch::kFloat32 || t == torch::kBFloat16;
+  };
+  TORCH_CHECK(real(pt) && real(gt),
+              "adamw: parameters and gradients must be float32 or bfloat16");
+  const auto state = eight ? torch::kFloat8_e4m3fn : torch::kFloat32;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  written.reserve(count * (eight ? 5 : 3));
+  auto check = [&](const torch::Tensor& t, torch::ScalarType type, int64_t n,
+                   bool out, const char* name) {
+    TORCH_CHECK(t.device() == dev, "adamw: ", name, " is on ", t.device(),
+                ", the first parameter on ", dev);
+    TORCH_CHECK(t.scalar_type() == type, "adamw: ", name, " must be ", type,
+                ", not ", t.scalar_type());
+    TORCH_CHECK(t.is_contiguous() && t.numel() == n, "adamw: ", name,
+                " must be contiguous with ", n, " elements");
+    if (out && n > 0) {
+      const auto a = reinterpret_cast<uintptr_t>(t.data_ptr());
+      written.emplace_back(a, a + t.nbytes());
+    }
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const int64_t n = p[i].numel();
+    check(p[i], pt, n, true, "a parameter");
+    check(g[i], gt, n, false, "a gradient");
+    check(m[i], state, n, true, "a first moment");
+    check(v[i], state, n, true, "a second moment");
+    if (eight) {
+      const int64_t blocks = (n + kAdamwBlock - 1) / kAdamwBlock;
+      check(ms[i], torch::kFloat32, blocks, true, "a first moment's scales");
+      check(vs[i], torch::kFloat32, blocks, true, "a second moment's scales");
+    }
+    if (prox) check(ref[i], torch::kFloat32, n, false, "a reference");
+  }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    TORCH_CHECK(written[i - 1].second <= written[i].first,
+                "adamw: a tensor that the step writes is there twice, or two "
+                "of them overlap");
+  AdamwScalars sc{};
+  sc.b1 = static_cast<float>(b1);
+  sc.omb1 = static_cast<float>(1.0 - b1);
+  sc.b2 = static_cast<float>(b2);
+  sc.omb2 = static_cast<float>(1.0 - b2);
+  sc.eps = static_cast<float>(eps);
+  sc.mu = static_cast<float>(mu);
+  sc.step = static_cast<float>(step);
+  sc.inv_bc2 = static_cast<float>(inv_bc2);
+  if (live.has_value()) {
+    check_gpu(*live, dev, "adamw: the live scalars");
+    TORCH_CHECK(live->scalar_type() == torch::kFloat32 &&
+                    live->is_contiguous() && live->numel() == 2,
+                "adamw: the live scalars are two contiguous float32");
+    sc.live = live->data_ptr<float>();
+  }
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  AdamwTable tab{};
+  int64_t grid = 0;
+  auto flush = [&] {
+    if (tab.count > 0) {
+      launch_adamw(tab, sc, pt == torch::kBFloat16, gt == torch::kBFloat16,
+                   eight, prox, stream());
+      HIP_CHECK_LAST();
+    }
+    tab.count = 0;
+    tab.aligned = 0;
+    grid = 0;
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const int64_t n = p[i].numel();
+    if (n == 0) continue;
+    const int64_t groups = (n + kAdamwChunk - 1) / kAdamwChunk;
+    TORCH_CHECK(groups < std::numeric_limits<int>::max(),
+                "adamw: a tensor of ", n, " elements is too long");
+    if (tab.count == kAdamwTensors ||
+        grid + groups > std::numeric_limits<int>::max())
+      flush();
+    AdamwTensor& t = tab.t[tab.count];
+    t.p = p[i].data_ptr();
+    t.g = g[i].data_ptr();
+    t.m = m[i].data_ptr();
+    t.v = v[i].data_ptr();
+    t.ms = eight ? ms[i].data_ptr<float>() : nullptr;
+    t.vs = eight ? vs[i].data_ptr<float>() : nullptr;
+    t.ref = prox ? ref[i].data_ptr<float>() : nullptr;
+    t.n = n;
+    // four elements at once: 16 bytes of fp32, 8 of bf16, 4 of codes
+    auto at = [](const void* q, size_t unit) {
+      return reinterpret_cast<uintptr_t>(q) % (4 * unit) == 0;
+    };
+    const size_t su = eight ? 1 : 4;
+    if (at(t.p, p[i].element_size()) && at(t.g, g[i].element_size()) &&
+        at(t.m, su) && at(t.v, su) && (!prox || at(t.ref, 4)))
+      tab.aligned |= 1ull << tab.count;
+    tab.keep[tab.count] = static_cast<float>(keep[i]);
+    tab.first[tab.count] = static_cast<int>(grid);
+    grid += groups;
+    tab.first[++tab.count] = static_cast<int>(grid);
+  }
+  flush();
+}
+
+// ---- residual add + layer norm ----------------------------------------------
+void check_norm(const torch::Tensor& x, const torch::Tensor& w,
+                int64_t groups, int64_t* rows, int64_t* H) {
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.is_contiguous(),
+              "add_norm: x must be a contiguous GPU tensor");
+  *H = x.size(-1);
+  TORCH_CHECK(*H >= 1 && *H <= kAddNormMaxH, "add_norm: rows of 1 to ",
+              kAddNormMaxH, " elements, not ", *H);
+  *rows = x.numel() / *H;
+  TORCH_CHECK(groups >= 1 && groups <= 65535 && *rows % groups == 0,
+              "add_norm: ", *rows, " rows do not divide into ", groups,
+              " groups");
+  TORCH_CHECK(*rows < std::numeric_limits<int>::max(),
+              "add_norm: too many rows");
+  check_gpu(w, x.device(), "add_norm: weight");
+  TORCH_CHECK(w.scalar_type() == torch::kFloat32 && w.is_contiguous() &&
+                  w.numel() == groups * *H,
+              "add_norm: weight and bias must be contiguous float32 with ",
+              groups * *H, " elements");
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>
+add_norm_fwd(torch::Tensor x, OptTensor r, torch::Tensor w, torch::Tensor b,
+             double eps, int64_t groups) {
+  int64_t rows, H;
+  const Elem type = elem_of(x, "add_norm: x");
+  check_norm(x, w, groups, &rows, &H);
+  check_norm(x, b, groups, &rows, &H);
+  if (r.has_value()) {
+    check_like(*r, x, "add_norm: residual");
+    TORCH_CHECK(r->is_contiguous(), "add_norm: residual must be contiguous");
+  }
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  auto y = torch::empty_like(x);
+  auto s = r.has_value() ? torch::empty_like(x) : x;
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  auto mean = torch::empty({rows}, f32), inv = torch::empty({rows}, f32);
+  if (rows == 0) return {y, s, mean, inv};
+  AddNormFwd f{};
+  f.x = x.data_ptr();
+  f.r = r.has_value() ? r->data_ptr() : nullptr;
+  f.w = w.data_ptr<float>();
+  f.b = b.data_ptr<float>();
+  f.s = s.data_ptr();
+  f.y = y.data_ptr();
+  f.mean = mean.data_ptr<float>();
+  f.inv = inv.data_ptr<float>();
+  f.rows = rows;
+  f.groups = static_cast<int>(groups);
+  f.H = static_cast<int>(H);
+  f.eps = static_cast<float>(eps);
+  const bool vec = H % 4 == 0 && aligned16(x) && aligned16(w) &&
+                   aligned16(b) && (!r.has_value() || aligned16(*r));
+  launch_add_norm_fwd(f, type, vec, stream());
+  HIP_CHECK_LAST();
+  return {y, s, mean, inv};
+}
+
+torch::Tensor add_norm_bwd(torch::Tensor gy, OptTensor gs, torch::Tensor s,
+                           torch::Tensor w, torch::Tensor mean,
+                           torch::Tensor inv, int64_t groups,
+                           torch::Tensor dw, torch::Tensor db) {
+  int64_t rows, H;
+  const Elem type = elem_of(s, "add_norm: the sum");
+  check_norm(s, w, groups, &rows, &H);
+  check_norm(s, dw, groups, &rows, &H);
+  check_norm(s, db, groups, &rows, &H);
+  check_like(gy, s, "add_norm: the output's gradient");
+  TORCH_CHECK(gy.is_contiguous(), "add_norm: gradients must be contiguous");
+  if (gs.has_value()) {
+    check_like(*gs, s, "add_norm: the sum's gradient");
+    TORCH_CHECK(gs->is_contiguous(), "add_norm: gradients must be contiguous");
+  }
+  for (const auto& t : {mean, inv}) {
+    check_gpu(t, s.device(), "add_norm: row statistics");
+    TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous() &&
+                    t.numel() == rows,
+                "add_norm: row statistics must be ", rows, " float32");
+  }
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(s.device());
+  auto gx = torch::empty_like(s);
+  if (rows == 0) {
+    dw.zero_();
+    db.zero_();
+    return gx;
+  }
+  const int parts =
+      add_norm_parts(rows, static_cast<int>(groups), static_cast<int>(H));
+  auto partials = torch::empty({groups, parts, 2, H},
+                               s.options().dtype(torch::kFloat32));
+  AddNormBwd b{};
+  b.gy = gy.data_ptr();
+  b.gs = gs.has_value() ? gs->data_ptr() : nullptr;
+  b.s = s.data_ptr();
+  b.w = w.data_ptr<float>();
+  b.mean = mean.data_ptr<float>();
+  b.inv = inv.data_ptr<float>();
+  b.gx = gx.data_ptr();
+  b.dw = dw.data_ptr<float>();
+  b.db = db.data_ptr<float>();
+  b.partials = partials.data_ptr<float>();
+  b.rows = rows;
+  b.groups = static_cast<int>(groups);
+  b.H = static_cast<int>(H);
+  b.parts = parts;
+  const bool vec = H % 4 == 0 && aligned16(s) && aligned16(w) &&
+                   aligned16(gy) && (!gs.has_value() || aligned16(*gs));
+  launch_add_norm_bwd(b, type, vec, stream());
+  HIP_CHECK_LAST();
+  return gx;
+}
+
+// ---- masked attention ---------------------------------------------------------
+// The kernels read 16 bytes at a time: rows of contiguous elements whose
+// strides and start are multiples of 8 of them.  Anything else is copied.
+torch::Tensor readable(const torch::Tensor& t) {
+  bool ok = t.stride(3) == 1 && aligned16(t);
+  for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
+  return ok ? t : t.contiguous();
+}
+
+HeadView view_of(const torch::Tensor& t) {
+  return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+}
+
+MaskedAttn describe(const torch::Tensor& q, const torch::Tensor& k,
+                    const torch::Tensor& v, double scale, bool causal,
+                    double softcap, const OptTensor& prefix,
+                    const OptTensor& doc, const OptTensor& slopes) {
+  TORCH_CHECK(q.is_cuda() && (q.scalar_type() == torch::kBFloat16 ||
+                              q.scalar_type() == torch::kFloat16),
+              "masked_attn: q must be a bfloat16 or float16 GPU tensor");
+  for (const auto& t : {k, v}) {
+    check_gpu(t, q.device(), "masked_attn: k and v");
+    TORCH_CHECK(t.scalar_type() == q.scalar_type(),
+                "masked_attn: q, k and v must have one type");
+  }
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() &&
+                  q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+                  q.size(3) == k.size(3),
+              "masked_attn: q [N, S, H, D] and k, v [N, S, Hkv, D] do not "
+              "match: ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+  const int64_t N = q.size(0), S = q.size(1), H = q.size(2), Hkv = k.size(2),
+                D = q.size(3);
+  TORCH_CHECK(Hkv >= 1 && H % Hkv == 0, "masked_attn: ", H,
+              " heads do not divide over ", Hkv, " key heads");
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0,
+              "masked_attn: head sizes are multiples of 8 up to 128, not ", D);
+  constexpr int64_t kMost = std::numeric_limits<int>::max();
+  TORCH_CHECK(S <= kMost - 256 && N <= kMost &&
+                  N * H * ((S + 63) / 64) <= kMost,
+              "masked_attn: too many tokens");
+  TORCH_CHECK(scale > 0.0 && softcap >= 0.0,
+              "masked_attn: the scale must be positive, the cap not negative");
+  MaskedAttn a{};
+  a.N = static_cast<int>(N);
+  a.S = static_cast<int>(S);
+  a.H = static_cast<int>(H);
+  a.Hkv = static_cast<int>(Hkv);
+  a.D = static_cast<int>(D);
+  a.causal = causal;
+  a.scale = static_cast<float>(scale);
+  a.softcap = static_cast<float>(softcap);
+  if (prefix.has_value()) {
+    check_gpu(*prefix, q.device(), "masked_attn: prefix");
+    TORCH_CHECK(prefix->scalar_type() == torch::kInt32 &&
+                    prefix->is_contiguous() && prefix->numel() == N,
+                "masked_attn: prefix must be int32 [", N, "]");
+    a.prefix = prefix->data_ptr<int>();
+  }
+  if (doc.has_value()) {
+    check_gpu(*doc, q.device(), "masked_attn: doc");
+    TORCH_CHECK(doc->scalar_type() == torch::kInt32 &&
+                    doc->is_contiguous() && doc->dim() == 2 &&
+                    doc->size(0) == N && doc->size(1) == S,
+                "masked_attn: doc must be contiguous int32 [", N, ", ", S,
+                "]");
+    a.doc = doc->data_ptr<int>();
+  }
+  if (slopes.has_value()) {
+    check_gpu(*slopes, q.device(), "masked_attn: slopes");
+    TORCH_CHECK(slopes->scalar_type() == torch::kFloat32 &&
+                    slopes->is_contiguous() && slopes->numel() == H,
+                "masked_attn: slopes must be float32 [", H, "]");
+    a.slopes = slopes->data_ptr<float>();
+  }
+  return a;
+}
+
+// (o [N, S, H, D], row statistics, summary of doc: empty if there is none)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> masked_attn_fwd(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale,
+    bool causal, double softcap, OptTensor prefix, OptTensor doc,
+    OptTensor slopes) {
+  MaskedAttn a =
+      describe(q, k, v, scale, causal, softcap, prefix, doc, slopes);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  auto o = torch::empty({a.N, a.S, a.H, a.D}, q.options());
+  auto lse = torch::empty({a.N, a.H, a.S}, q.options().dtype(torch::kFloat32));
+  // A summary costs a launch; up to four tiles a row testing every pair is
+  // cheaper.
+  const int64_t tiles = (a.S + kAttnTile - 1) / kAttnTile;
+  const bool summary = doc.has_value() && tiles > 4;
+  auto sum = torch::empty({summary ? a.N * tiles : 0, 4},
+                          q.options().dtype(torch::kInt32));
+  if (o.numel() == 0) return {o, lse, sum};
+  q = readable(q);
+  k = readable(k);
+  v = readable(v);
+  a.q = view_of(q);
+  a.k = view_of(k);
+  a.v = view_of(v);
+  a.o = view_of(o);
+  a.lse = lse.data_ptr<float>();
+  if (summary) {
+    a.tiles = reinterpret_cast<int4*>(sum.data_ptr<int>());
+    launch_masked_attn_tiles(a, stream());
+  }
+  launch_masked_attn_fwd(a, elem_of(q, "q"), stream());
+  HIP_CHECK_LAST();
+  return {o, lse, sum};
+}
+
+// Writes gq, gk, gv: any layout whose rows are contiguous and whose strides
+// and start are multiples of 8 elements.
+void masked_attn_bwd(torch::Tensor go, torch::Tensor q, torch::Tensor k,
+                     torch::Tensor v, torch::Tensor o, torch::Tensor lse,
+                     torch::Tensor sum, torch::Tensor gq, torch::Tensor gk,
+                     torch::Tensor gv, double scale, bool causal,
+                     double softcap, OptTensor prefix, OptTensor doc,
+                     OptTensor slopes) {
+  MaskedAttn a =
+      describe(q, k, v, scale, causal, softcap, prefix, doc, slopes);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  check_like(go, q, "masked_attn: the output's gradient");
+  check_like(o, q, "masked_attn: the output");
+  check_like(gq, q, "masked_attn: q's gradient");
+  check_like(gk, k, "masked_attn: k's gradient");
+  check_like(gv, v, "masked_attn: v's gradient");
+  check_gpu(lse, q.device(), "masked_attn: row statistics");
+  check_gpu(sum, q.device(), "masked_attn: summary");
+  const int64_t tiles = (a.S + kAttnTile - 1) / kAttnTile;
+  TORCH_CHECK(lse.scalar_type() == torch::kFloat32 && lse.is_contiguous() &&
+                  lse.numel() == static_cast<int64_t>(a.N) * a.H * a.S,
+              "masked_attn: row statistics do not match");
+  TORCH_CHECK(sum.scalar_type() == torch::kInt32 && sum.is_contiguous() &&
+                  (sum.numel() == 0 ||
+                   (doc.has_value() && sum.numel() == a.N * tiles * 4)),
+              "masked_attn: the summary does not match");
+  for (const auto& t : {gq, gk, gv}) {
+    bool ok = t.stride(3) == 1 && aligned16(t);
+    for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
+    TORCH_CHECK(ok, "masked_attn: gradients need contiguous rows at 16 bytes");
+  }
+  if (q.numel() == 0) {
+    gk.zero_();
+    gv.zero_();
+    return;
+  }
+  q = readable(q);
+  k = readable(k);
+  v = readable(v);
+  go = readable(go);
+  o = readable(o);
+  auto delta = torch::empty_like(lse);
+  a.q = view_of(q);
+  a.k = view_of(k);
+  a.v = view_of(v);
+  a.o = view_of(o);
+  a.go = view_of(go);
+  a.gq = view_of(gq);
+  a.gk = view_of(gk);
+  a.gv = view_of(gv);
+  a.lse = lse.data_ptr<float>();
+  a.delta = delta.data_ptr<float>();
+  if (sum.numel() > 0) a.tiles = reinterpret_cast<int4*>(sum.data_ptr<int>());
+  launch_masked_attn_bwd(a, elem_of(q, "q"), stream());
+  HIP_CHECK_LAST();
+}
+
+}  // namespace
+
+void bind_encoder(pybind11::module& m) {
+  m.def("adamw_step", &adamw_step);
+  m.def("add_norm_fwd", &add_norm_fwd);
+  m.def("add_norm_bwd", &add_norm_bwd);
+  m.def("masked_attn_fwd", &masked_attn_fwd);
+  m.def("masked_attn_bwd", &masked_attn_bwd);
+}
+
+}  // namespace colearn

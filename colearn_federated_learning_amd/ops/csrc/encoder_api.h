@@ -1,0 +1,112 @@
+// Launchers of the encoder-training kernels (adamw.hip, add_norm.hip,
+// masked_attn.hip), shared with bindings_encoder.cpp.
+#pragma once
+
+#include <hip/hip_runtime_api.h>
+
+#include <cstdint>
+
+namespace colearn {
+
+enum class Elem : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+// ---- AdamW over many tensors ----------------------------------------------
+constexpr int kAdamwTensors = 48;   // tensors a launch; the table is passed by
+                                    // value and has to fit 4 KB of arguments
+constexpr int kAdamwBlock = 256;    // elements that share one 8-bit scale
+constexpr int kAdamwChunk = 2048;   // elements a workgroup
+
+struct AdamwTensor {
+  void* p;
+  const void* g;
+  void* m;  // fp32, or e4m3 codes
+  void* v;  // fp32, or e4m3 codes of the root
+  float* ms;
+  float* vs;  // scales, one a block (8-bit only)
+  const float* ref;
+  int64_t n;
+};
+
+struct AdamwTable {
+  AdamwTensor t[kAdamwTensors];
+  float keep[kAdamwTensors];       // 1 - lr * weight decay
+  int first[kAdamwTensors + 1];    // first workgroup of each tensor
+  unsigned long long aligned;      // bit i: tensor i takes vector accesses
+  int count;
+};
+
+struct AdamwScalars {
+  float b1, omb1, b2, omb2, eps, mu, step, inv_bc2;
+  const float* live;  // [step, inv_bc2] on the device, or null
+};
+
+void launch_adamw(const AdamwTable& t, const AdamwScalars& s, bool p_bf16,
+                  bool g_bf16, bool eight, bool prox, hipStream_t stream);
+
+// ---- residual add + layer norm ----------------------------------------------
+constexpr int kAddNormMaxH = 16384;
+
+struct AddNormFwd {
+  const void* x;
+  const void* r;  // or null
+  const float* w;
+  const float* b;
+  void* s;  // written if r is there
+  void* y;
+  float* mean;
+  float* inv;
+  int64_t rows;
+  int groups, H;
+  float eps;
+};
+
+struct AddNormBwd {
+  const void* gy;
+  const void* gs;  // gradient of the sum itself, or null
+  const void* s;
+  const float* w;
+  const float* mean;
+  const float* inv;
+  void* gx;
+  float* dw;
+  float* db;
+  float* partials;  // [groups][parts][2][H]
+  int64_t rows;
+  int groups, H, parts;
+};
+
+int add_norm_parts(int64_t rows, int groups, int H);
+void launch_add_norm_fwd(const AddNormFwd& f, Elem type, bool vec,
+                         hipStream_t stream);
+void launch_add_norm_bwd(const AddNormBwd& b, Elem type, bool vec,
+                         hipStream_t stream);
+
+// ---- masked attention ---------------------------------------------------------
+constexpr int kAttnTile = 64;  // tokens a tile of the mask's summary
+
+struct HeadView {  // [N, S, heads, D] with D contiguous
+  void* p;
+  int64_t sn, ss, sh;
+};
+
+struct MaskedAttn {
+  HeadView q, k, v, o;        // o: [N, S, H, D]
+  HeadView go, gq, gk, gv;    // backward only
+  const int* doc;             // [N, S], or null
+  const int* prefix;          // [N], or null
+  const float* slopes;        // [H], or null
+  int4* tiles;                // [N, ceil(S / 64)] summary of doc, or null
+  float* lse;                 // [N, H, S], base 2; +inf for empty rows
+  float* delta;               // [N, H, S], backward only
+  int N, S, H, Hkv, D;
+  bool causal;
+  float scale, softcap;
+};
+
+void launch_masked_attn_tiles(const MaskedAttn& a, hipStream_t stream);
+void launch_masked_attn_fwd(const MaskedAttn& a, Elem type,
+                            hipStream_t stream);
+void launch_masked_attn_bwd(const MaskedAttn& a, Elem type,
+                            hipStream_t stream);
+
+}  // namespace colearn

@@ -11,6 +11,8 @@ inputs may be bf16, parameters stay fp32.
 
 from __future__ import annotations
 
+from typing import Optional, Tuple
+
 import torch
 import torch.nn as nn
 
@@ -271,3 +273,118 @@ class ColearnLayerNorm(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         y, _, _ = _LayerNormFn.apply(x, self.weight, self.bias, self.eps)
         return y
+
+
+def _add_layer_norm_ref(x, residual, weight, bias, eps, groups):
+    """The same formulas in torch (differentiable): CPU tensors, float64,
+    functorch transforms; the kernel's oracle."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    # gradients of both outputs meet in the wide sum and are rounded once;
+    # what is normalised has the rounded sum's value
+    t = x.to(wide)
+    if residual is not None:
+        t = t + residual.to(wide)
+    s = t.to(x.dtype)
+    h = (t + (s.to(wide) - t).detach()).reshape(groups, -1, x.shape[-1])
+    mean = h.mean(dim=-1, keepdim=True)
+    c = h - mean
+    inv = (c.square().mean(dim=-1, keepdim=True) + eps).rsqrt()
+    y = (c * inv * weight.reshape(groups, 1, -1)
+         + bias.reshape(groups, 1, -1))
+    return y.to(x.dtype).reshape(x.shape), s
+
+
+class _AddLayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, groups, gslot_w,
+                gslot_b):
+        y, s, mean, inv = require_ext().add_norm_fwd(
+            x, residual, weight, bias, eps, groups)
+        ctx.save_for_backward(s, weight, mean, inv)
+        ctx.groups = groups
+        ctx.gslots = (gslot_w, gslot_b)
+        ctx.bias_shape = bias.shape
+        ctx.set_materialize_grads(False)
+        if residual is None:
+            s = s.view_as(s)  # an input is not an output of its own
+        return y, s
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy, gs):
+        s, weight, mean, inv = ctx.saved_tensors
+        if gy is None:  # only the sum was used
+            return (gs, gs if ctx.needs_input_grad[1] else None, None, None,
+                    None, None, None, None)
+        gw, gb = ctx.gslots
+        direct = gw is not None
+        if not direct:
+            gw = torch.empty_like(weight)
+            gb = torch.empty(ctx.bias_shape, dtype=weight.dtype,
+                             device=weight.device)
+        gx = require_ext().add_norm_bwd(
+            gy.contiguous(), None if gs is None else gs.contiguous(), s,
+            weight, mean, inv, ctx.groups, gw, gb)
+        if direct:
+            gw = gb = None
+        return (gx, gx if ctx.needs_input_grad[1] else None, gw, gb, None,
+                None, None, None)
+
+
+def colearn_add_layer_norm(
+    x: torch.Tensor, residual: Optional[torch.Tensor],
+    weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-12,
+    groups: int = 1, gslot_w: Optional[torch.Tensor] = None,
+    gslot_b: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(LayerNorm(s), s)`` with ``s = x + residual`` (``x`` itself without a
+    residual), over the last dimension: the join of a transformer block and
+    its norm in one pass.  ``s`` has x's type, and what is normalised is the
+    rounded ``s``; both outputs take gradients.
+
+    ``groups`` > 1: stacked clients, rows client-major, ``weight`` and ``bias``
+    [groups, H].  ``gslot_w`` / ``gslot_b`` (both or none, float32, weight's
+    size, contiguous): the backward writes the parameters' gradients there
+    (overwriting them) and returns none, as the stacked engine's norms do.
+
+    float32, bfloat16 and float16 on the GPU, rows up to 16384, run the HIP
+    kernels (csrc/add_norm.hip); the parameters are float32.  Other operands
+    run the same formulas in torch (without gslots).  A residual of another
+    type is joined in the wider of the two.
+    """
+    h = x.shape[-1] if x.dim() else 0
+    if h < 1 or weight.numel() != groups * h or bias.numel() != groups * h:
+        raise ValueError(
+            f"weight and bias must have {groups} x {h} elements, got "
+            f"{tuple(weight.shape)} and {tuple(bias.shape)}")
+    if groups < 1 or (x.numel() // h) % groups:
+        raise ValueError(f"{x.numel() // h} rows do not divide into {groups} "
+                         f"groups")
+    if not x.is_floating_point():
+        raise TypeError(f"x must be floating, got {x.dtype}")
+    if (gslot_w is None) != (gslot_b is None):
+        raise ValueError("gslot_w and gslot_b go together")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"the residual's shape {tuple(residual.shape)} "
+                             f"is not x's {tuple(x.shape)}")
+        if residual.dtype != x.dtype:
+            dt = torch.promote_types(x.dtype, residual.dtype)
+            x, residual = x.to(dt), residual.to(dt)
+    for t in (residual, weight, bias):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"operands on {x.device} and {t.device}")
+    native = (x.is_cuda and native_enabled() and not is_vmapped(x, weight)
+              and x.dtype in (torch.float32, torch.bfloat16, torch.float16)
+              and h <= 16384)
+    if not native:
+        if gslot_w is not None:
+            raise ValueError("gslots need the native kernel")
+        return _add_layer_norm_ref(x, residual, weight, bias, eps, groups)
+    if weight.dtype != torch.float32 or bias.dtype != torch.float32:
+        raise TypeError("weight and bias must be float32")
+    return _AddLayerNormFn.apply(
+        x.contiguous(),
+        None if residual is None else residual.contiguous(),
+        weight.contiguous(), bias.contiguous(), eps, groups, gslot_w,
+        gslot_b)

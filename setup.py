@@ -26,6 +26,10 @@ ext = CUDAExtension(
     name="colearn_federated_learning_amd.ops._colearn_hip",
     sources=[
         os.path.join(CSRC, "bindings.cpp"),
+        os.path.join(CSRC, "bindings_encoder.cpp"),
+        os.path.join(CSRC, "adamw.hip"),
+        os.path.join(CSRC, "add_norm.hip"),
+        os.path.join(CSRC, "masked_attn.hip"),
         os.path.join(CSRC, "fused_optim.hip"),
         os.path.join(CSRC, "dp_topk.hip"),
         os.path.join(CSRC, "norms.hip"),
