@@ -303,6 +303,8 @@ torch::Tensor add_norm_bwd(torch::Tensor gy, OptTensor gs, torch::Tensor s,
 torch::Tensor readable(const torch::Tensor& t) {
   bool ok = t.stride(3) == 1 && aligned16(t);
   for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
+  // a tile's rows are addressed with 32 bits
+  ok = ok && t.stride(1) >= 0 && t.stride(1) <= (1 << 24);
   return ok ? t : t.contiguous();
 }
 

@@ -103,6 +103,8 @@ struct MaskedAttn {
   float scale, softcap;
 };
 
+// whether two waves share 32 owned tokens, for a grid of `heads` a sequence
+bool masked_attn_split(const MaskedAttn& a, int heads);
 void launch_masked_attn_tiles(const MaskedAttn& a, hipStream_t stream);
 void launch_masked_attn_fwd(const MaskedAttn& a, Elem type,
                             hipStream_t stream);

@@ -1,0 +1,471 @@
+// Self-attention with document masks, causal and prefix masks, capped scores
+// and linear distance biases, for any length; forward and backward, bf16 or
+// fp16 operands, head sizes up to 128, shared key heads.
+//
+//   z_ij = scale q_i.k_j;  z = cap tanh(z / cap);  z -= slope_h |i - j|
+//   (i, j) attended:  doc_i == doc_j >= 0  and  (not causal or j <= i or
+//                     j < prefix)
+//   p = softmax of z over the attended j (all 0 if there is none),  o = p v
+//   D_i = go_i.o_i;  dp = go v^T;  dz = p (dp - D) (1 - tanh^2)
+//   dq = scale dz k,  dk = scale dz^T q,  dv = p^T go
+//
+// All three kernels have one shape.  A wave owns 32 tokens (queries in the
+// forward and dq kernels, keys in the dk/dv kernel) whose operands stay in
+// registers, and tiles of 64 tokens of the other side stream through LDS,
+// double-buffered: the next tile's loads are issued before a tile is worked
+// on and land in the other buffer after it.  A workgroup's four waves own 128
+// tokens (KS = 1), or 64 with two waves on each 32, one for either half of
+// every tile, joined through LDS at the end (KS = 2).  Products are 32x32x16 MFMAs with
+// the streamed side as the left operand, so that a lane's column of the
+// result belongs to one owned token and its 16 registers to streamed tokens:
+// the softmax is a reduction over registers plus one exchange between the
+// wave's halves, and the rounded probabilities already lie as the right
+// operand of the second product.  That operand's k order is
+//     slot 8h + j  <->  token 4h + (j & 3) + 8 (j >> 2)       (h: lane / 32)
+// instead of the plain one; the left operand, read transposed from the same
+// LDS tile (ds_read_b64_tr_b16: four tokens of 16 columns a lane group), uses
+// the same order, so nothing moves between lanes.
+//
+// In fp16 the backward rounds 2^15 p instead of p (the factor leaves dv again
+// in fp32): a uniform row of 16K tokens has p = 2^-14, below which fp16 loses
+// a bit for every halving.  dz has no such bound and is rounded as it is.
+//
+// Scores are held in base 2 (scale * log2 e folded in) and every statistic in
+// fp32.  Probabilities and dz are rounded to the operands' type for the second
+// products; the sums in the denominator are of the unrounded ones.
+//
+// The mask is summarised per 64 tokens (smallest and largest document, any
+// padding).  A workgroup first lists the tiles that it has to visit, each
+// marked whole (every pair attended: no test in the loop) or mixed; tiles
+// between documents that do not meet cost nothing.  Rows of padding are
+// staged as zeros and rows of padding are written as zeros, so that whatever
+// a padded token holds reaches no result.
+//
+// The backward recomputes p from the saved row statistic, in two kernels
+// without atomics (dq with D, then dk/dv): 7 products instead of the 5 of a
+// single kernel whose dq would be summed by atomics in an order that changes
+// from run to run.
+#pragma once
+
+#include <type_traits>
+
+#include "elem.h"
+#include "encoder_api.h"
+
+namespace colearn {
+
+namespace masked_attn {
+
+constexpr int kTile = kAttnTile;   // streamed tokens a tile
+constexpr int kList = 1024;        // tiles listed at a time
+constexpr float kLog2e = 1.4426950408889634f;
+
+// What happens to a score before the exponential, besides its scale
+enum Mode : int { kPlain = 0, kBias = 1, kCap = 2 };  // kCap: bias too, if any
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <typename T>
+DEV_INLINE f32x16 mfma(s16x8 a, s16x8 b, f32x16 c);
+template <>
+DEV_INLINE f32x16 mfma<bf16>(s16x8 a, s16x8 b, f32x16 c) {
+  typedef __attribute__((ext_vector_type(8))) __bf16 V;
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+      __builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+}
+template <>
+DEV_INLINE f32x16 mfma<f16>(s16x8 a, s16x8 b, f32x16 c) {
+  typedef __attribute__((ext_vector_type(8))) _Float16 V;
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+      __builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+}
+
+// registers 8k .. 8k+7 of a result, rounded to T
+template <typename T>
+DEV_INLINE s16x8 round8(const f32x16& x, int k) {
+  typedef __attribute__((ext_vector_type(8))) typename Bits16<T>::hw V;
+  f32x8 f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = x[8 * k + j];
+  return __builtin_bit_cast(s16x8, __builtin_convertvector(f, V));
+}
+
+// what a probability is multiplied with before it is rounded, in the backward
+template <typename T>
+constexpr float kLift = std::is_same<T, f16>::value ? 32768.f : 1.f;
+
+DEV_INLINE float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh from one exponential and one reciprocal; off by about 1e-7, far below
+// the rounding of the products around it
+DEV_INLINE float fast_tanh(float x) {
+  const float e = fast_exp2(x * (2.f * kLog2e));
+  return 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+}
+
+// the other half's value (lane ^ 32)
+DEV_INLINE float other_half(float x) { return __shfl_xor(x, 32); }
+
+// A tile of kTile rows of DP 16-bit values.  16-byte slots are permuted
+// within a row so that neither read below hits a bank twice: eight
+// consecutive rows of a slot (row operand) lie over all slots of 128 bytes,
+// and so do four consecutive rows of two slots (transposed operand).
+template <int DP>
+struct Tile {
+  static constexpr int kSlots = DP / 8;
+  static constexpr int kStep = 256 / kSlots;       // rows a pass of all threads
+  static constexpr int kPer = kTile / kStep;       // passes
+  static constexpr int kBytes = kTile * DP * 2;
+
+  DEV_INLINE static int at(int row, int slot) {
+    const int f = DP == 32 ? ((row & 2) | ((row >> 2) & 1))
+                           : (((row & 3) << 1) | ((row >> 2) & 1));
+    return row * (DP * 2) + ((slot ^ f) << 4);
+  }
+
+  // left operand: rows 0..31 of `half` (32 rows), columns 16 kk + 0..15
+  DEV_INLINE static s16x8 rows(const char* half, int kk) {
+    const int lane = threadIdx.x % kWave;
+    return *reinterpret_cast<const s16x8*>(
+        half + at(lane & 31, kk * 2 + (lane >> 5)));
+  }
+  // transposed left operand: columns 32 db + 0..31 as rows, tokens 16 ks +
+  // 0..15 of `half` in the order of the file's head
+  DEV_INLINE static s16x8 cols(const char* half, int ks, int db) {
+    const int lane = threadIdx.x % kWave;
+    const int i = lane & 15;
+    const int row = ((lane >> 5) << 2) + (i >> 2);
+    const int slot = db * 4 + ((lane >> 4) & 1) * 2 + ((i >> 1) & 1);
+    const char* p = half + at(row, slot) + (i & 1) * 8 + ks * (16 * DP * 2);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(p + 8 * DP * 2));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// One streamed operand [S, D]: this thread's 16 bytes of a tile's rows
+// threadIdx.x / kSlots + i kStep.  The row's offset in a tile is 32 bits (the
+// host sees to it), the tile's own 64.
+template <int DP>
+struct Stream {
+  using L = Tile<DP>;
+  const short* base;
+  int64_t ss;
+  unsigned off;
+
+  DEV_INLINE Stream(const short* p, int64_t stride, int D)
+      : base(p), ss(stride) {
+    const int slot = threadIdx.x % L::kSlots;
+    off = (threadIdx.x / L::kSlots) * static_cast<unsigned>(stride) +
+          (slot * 8 < D ? slot * 8 : 0);
+  }
+  DEV_INLINE void load(int t0, int S, s16x8 (&r)[L::kPer]) const {
+    const short* p = base + t0 * ss;
+    if (t0 + kTile <= S) {
+#pragma unroll
+      for (int i = 0; i < L::kPer; ++i)
+        r[i] = *reinterpret_cast<const s16x8*>(p + i * (L::kStep * ss) + off);
+    } else {
+#pragma unroll
+      for (int i = 0; i < L::kPer; ++i) {
+        const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+        r[i] = zero;
+        if (t0 + i * L::kStep + static_cast<int>(threadIdx.x) / L::kSlots < S)
+          r[i] =
+              *reinterpret_cast<const s16x8*>(p + i * (L::kStep * ss) + off);
+      }
+    }
+  }
+  // rows of padding and columns past D as zeros; live: bit i for pass i
+  DEV_INLINE static void store(char* lds, unsigned live, int D,
+                               const s16x8 (&r)[L::kPer]) {
+    const int row = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
+    const unsigned keep = slot * 8 < D ? live : 0;
+#pragma unroll
+    for (int i = 0; i < L::kPer; ++i) {
+      const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+      *reinterpret_cast<s16x8*>(lds + L::at(row + i * L::kStep, slot)) =
+          (keep >> i) & 1 ? r[i] : zero;
+    }
+  }
+};
+
+// documents of the rows that this thread stages: bit i set if row i is no
+// padding (rows past S are zeros already)
+template <int DP>
+DEV_INLINE unsigned live_rows(const int* doc, int t0, int S) {
+  using L = Tile<DP>;
+  if (doc == nullptr) return ~0u;
+  unsigned live = 0;
+#pragma unroll
+  for (int i = 0; i < L::kPer; ++i) {
+    const int tok =
+        min(t0 + i * L::kStep + static_cast<int>(threadIdx.x) / L::kSlots,
+            S - 1);
+    live |= (doc[tok] >= 0 ? 1u : 0u) << i;
+  }
+  return live;
+}
+
+// right operand of an owned token's row: columns 16 kk + 8 h + 0..7
+template <int DP>
+DEV_INLINE void own_rows(const short* row, bool live, int D,
+                         s16x8 (&r)[DP / 16]) {
+  const int h = (threadIdx.x % kWave) >> 5;
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int col = kk * 16 + h * 8;
+    const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    r[kk] = live && col < D ? *reinterpret_cast<const s16x8*>(row + col)
+                            : zero;
+  }
+}
+
+// a transposed result: this lane's token gets columns 32 db + (r & 3) +
+// 8 (r >> 2) + 4 h
+template <typename T, int DP>
+DEV_INLINE void store_cols(T* row, const f32x16 (&acc)[DP / 32], float f,
+                           bool live, int D) {
+  const int h = (threadIdx.x % kWave) >> 5;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = db * 32 + g * 8 + h * 4;
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = live ? acc[db][g * 4 + j] * f : 0.f;
+      if (col < D) elem_store4(row + col, x);
+    }
+}
+
+// What the pairs of tokens [q0, q1) x [k0, k1) are: 0 none attended, 1 some,
+// 2 all.  A tile that reaches past S counts as mixed on the key side only:
+// no query row past S is ever written, or has a statistic but +inf.
+DEV_INLINE int meet(bool causal, int prefix, int S, int q0, int q1, int k0,
+                    int k1, bool doc, int4 a, int4 b) {
+  int c = k1 > S ? 1 : 2;
+  const int qe = min(q1, S) - 1, ke = min(k1, S) - 1;
+  if (causal) {
+    if (k0 > qe && k0 >= prefix) return 0;
+    if (!(ke <= q0 || ke < prefix)) c = 1;
+  }
+  if (doc) {
+    if (a.x > b.y || b.x > a.y) return 0;
+    if (a.x != a.y || b.x != b.y || a.z || b.z) c = 1;
+  }
+  return c;
+}
+
+DEV_INLINE int4 join(int4 a, int4 b) {
+  return make_int4(min(a.x, b.x), max(a.y, b.y), a.z | b.z, 0);
+}
+
+// Lists the tiles of [base, base + kList) that meet the owned tokens from own0
+// on: (tile << 1) | whole, in order.  Called by the whole workgroup.
+template <bool OWN_Q, int OWN>
+DEV_INLINE int list_tiles(const MaskedAttn& a, int n, int own0, int base,
+                          int* list, int* count) {
+  const int tiles = (a.S + kTile - 1) / kTile;
+  __syncthreads();  // the previous list is used up
+  if (threadIdx.x < kWave) {
+    const int lane = threadIdx.x;
+    const int prefix = a.prefix != nullptr ? a.prefix[n] : 0;
+    const bool summary = a.tiles != nullptr;
+    const int4* row = a.tiles + static_cast<int64_t>(n) * tiles;
+    int4 mine = make_int4(0, 0, 0, 0);
+    if (summary) {
+      const int t = own0 / kTile;
+      mine = row[t];
+      if (OWN > kTile && t + 1 < tiles) mine = join(mine, row[t + 1]);
+    }
+    int found = 0;
+    const int end = min(base + kList, tiles);
+    for (int t0 = base; t0 < end; t0 += kWave) {
+      const int t = t0 + lane;
+      int c = 0;
+      if (t < end) {
+        const int4 other = summary ? row[t] : mine;
+        const int s0 = t * kTile;
+        c = OWN_Q ? meet(a.causal, prefix, a.S, own0, own0 + OWN, s0,
+                         s0 + kTile, summary, mine, other)
+                  : meet(a.causal, prefix, a.S, s0, s0 + kTile, own0,
+                         own0 + OWN, summary, mine, other);
+        if (c == 2 && a.doc != nullptr && !summary) c = 1;
+      }
+      const unsigned long long hit = __ballot(c != 0);
+      if (c != 0)
+        list[found + __popcll(hit & ((1ull << lane) - 1))] =
+            (t << 1) | (c == 2);
+      found += __popcll(hit);
+    }
+    if (lane == 0) *count = found;
+  }
+  __syncthreads();
+  return *count;
+}
+
+// document of a streamed token: -1 for padding and past the end, 0 without
+// documents
+DEV_INLINE int doc_of(const MaskedAttn& a, int n, int tok) {
+  if (tok >= a.S) return -1;
+  if (a.doc == nullptr) return 0;
+  return max(a.doc[static_cast<int64_t>(n) * a.S + tok], -1);
+}
+
+DEV_INLINE const short* row_of(const HeadView& v, int n, int h) {
+  return static_cast<const short*>(v.p) + n * v.sn + h * v.sh;
+}
+
+// block -> (sequence, head, owned tokens): one head's blocks stay on one XCD,
+// whose L2 then holds what they stream
+template <int OWN>
+DEV_INLINE void locate(const MaskedAttn& a, int heads, bool last_first,
+                       int* n, int* h, int* own0) {
+  const int blocks = (a.S + OWN - 1) / OWN;
+  const int total = gridDim.x;
+  const int q = total / kNumXCD, r = total % kNumXCD;
+  const int xcd = blockIdx.x % kNumXCD, idx = blockIdx.x / kNumXCD;
+  const int id =
+      (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+  const int nh = id / blocks;
+  int b = id % blocks;
+  if (last_first) b = blocks - 1 - b;  // causal: the longest rows first
+  *n = nh / heads;
+  *h = nh % heads;
+  *own0 = b * OWN;
+}
+
+// From q.k to what the exponential takes: p = exp2(c z - statistic), with z
+// -inf where the pair is masked.
+template <Mode M>
+struct Score {
+  float c;       // scale * log2 e, or cap * log2 e
+  float cap_in;  // scale / cap
+  float slope;   // slope * log2 e / c
+
+  DEV_INLINE Score(const MaskedAttn& a, int h) {
+    c = a.scale * kLog2e;
+    cap_in = 0.f;
+    if (M == kCap) {
+      cap_in = a.scale / a.softcap;
+      c = a.softcap * kLog2e;
+    }
+    slope = M != kPlain && a.slopes != nullptr ? a.slopes[h] * kLog2e / c
+                                               : 0.f;
+  }
+
+  // dist: owned token minus the streamed token of register 0
+  DEV_INLINE void shape(f32x16& z, float dist) const {
+    if constexpr (M == kCap) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = fast_tanh(z[r] * cap_in);
+    }
+    if constexpr (M != kPlain) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        z[r] -= slope * fabsf(dist - ((r & 3) + 8 * (r >> 2)));
+    }
+  }
+};
+
+// -inf where this lane's token and the streamed ones are not a pair.  doc: the
+// streamed tokens' documents from register 0's on; own_doc: -2 for a token
+// without any.  OWN_Q: the streamed token has to be at most `lim`, else at
+// least.  One test covers the causal mask and the prefix (pair_limit).
+template <bool OWN_Q>
+DEV_INLINE void mask(f32x16& z, int own_doc, int lim, int other0,
+                     const int* doc) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int4 d = *reinterpret_cast<const int4*>(doc + g * 8);
+    const int dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int tok = other0 + g * 8 + j;
+      const bool ok = (dd[j] == own_doc) & (OWN_Q ? tok <= lim : tok >= lim);
+      z[g * 4 + j] = ok ? z[g * 4 + j] : -INFINITY;
+    }
+  }
+}
+
+// OWN_Q: the last key that query `own` may attend to; else the first query
+// that may attend to key `own`
+template <bool OWN_Q>
+DEV_INLINE int pair_limit(const MaskedAttn& a, int n, int own) {
+  if (!a.causal) return OWN_Q ? 0x7fffffff : 0;
+  const int prefix = a.prefix != nullptr ? a.prefix[n] : 0;
+  if (OWN_Q) return max(own, prefix - 1);
+  return own < prefix ? 0 : own;
+}
+
+template <int DP>
+struct Smem {
+  char tile[2][2][Tile<DP>::kBytes];  // buffer, operand
+  int doc[2][kTile];
+  float lse[2][kTile];    // dk/dv only
+  float delta[2][kTile];  // dk/dv only
+  int list[kList];
+  int count;
+};
+
+// The two waves of 32 owned tokens (KS = 2) meet in the tile buffers: the
+// second leaves its registers, the first picks them up.
+template <int N>
+DEV_INLINE void leave(float* at, const f32x16 (&x)[N]) {
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) at[(i * 16 + r) * kWave + lane] = x[i][r];
+}
+template <int N>
+DEV_INLINE void pick_up(const float* at, f32x16 (&x)[N]) {
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[i][r] = at[(i * 16 + r) * kWave + lane];
+}
+
+inline Mode mode_of(const MaskedAttn& a) {
+  return a.softcap > 0.f ? kCap : a.slopes != nullptr ? kBias : kPlain;
+}
+
+// calls f.template run<T, DP, M>()
+template <typename F, typename T, int DP>
+void with_mode(const F& f, const MaskedAttn& a) {
+  switch (mode_of(a)) {
+    case kPlain:
+      return f.template run<T, DP, kPlain>();
+    case kBias:
+      return f.template run<T, DP, kBias>();
+    case kCap:
+      return f.template run<T, DP, kCap>();
+  }
+}
+template <typename F, typename T>
+void with_size(const F& f, const MaskedAttn& a) {
+  if (a.D <= 32)
+    with_mode<F, T, 32>(f, a);
+  else if (a.D <= 64)
+    with_mode<F, T, 64>(f, a);
+  else
+    with_mode<F, T, 128>(f, a);
+}
+template <typename F>
+void with_type(const F& f, const MaskedAttn& a, Elem type) {
+  if (type == Elem::kBF16)
+    with_size<F, bf16>(f, a);
+  else
+    with_size<F, f16>(f, a);
+}
+
+}  // namespace masked_attn
+
+}  // namespace colearn

@@ -1,0 +1,335 @@
+// Masked attention, backward.  The mathematics and the layout stand in
+// masked_attn.h.
+
+#include "masked_attn.h"
+
+namespace colearn {
+
+using namespace masked_attn;
+
+namespace {
+
+template <typename T, int DP, Mode M, int KS>
+__global__ __launch_bounds__(256, 2) void masked_attn_dq_kernel(
+    MaskedAttn a) {
+  using L = Tile<DP>;
+  constexpr int OWN = 128 / KS, KB = 2 / KS;
+  __shared__ __align__(16) Smem<DP> sm;
+  int n, h, own0;
+  locate<OWN>(a, a.H, a.causal, &n, &h, &own0);
+  const int hk = h / (a.H / a.Hkv);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
+  const int own = own0 + (wave / KS) * 32 + (lane & 31);
+  const int found = doc_of(a, n, own);
+  const bool live = found >= 0;
+  const int own_doc = live ? found : -2;
+  const int lim = pair_limit<true>(a, n, own);
+  const int* doc =
+      a.doc != nullptr ? a.doc + static_cast<int64_t>(n) * a.S : nullptr;
+  const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss, a.D);
+  const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss, a.D);
+  s16x8 qf[DP / 16], gf[DP / 16];
+  own_rows<DP>(row_of(a.q, n, h) + own * a.q.ss, live, a.D, qf);
+  own_rows<DP>(row_of(a.go, n, h) + own * a.go.ss, live, a.D, gf);
+  float delta = 0.f, lse = INFINITY;
+  {
+    const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S + own;
+    s16x8 of[DP / 16];
+    own_rows<DP>(row_of(a.o, n, h) + own * a.o.ss, live, a.D, of);
+    typedef __attribute__((ext_vector_type(8))) typename Bits16<T>::hw V;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      const V g = __builtin_bit_cast(V, gf[kk]);
+      const V o = __builtin_bit_cast(V, of[kk]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        delta += static_cast<float>(g[j]) * static_cast<float>(o[j]);
+    }
+    delta += other_half(delta);
+    if (own < a.S) {
+      lse = a.lse[stat];
+      if (half == 0 && part == 0) a.delta[stat] = delta;
+    }
+  }
+  const Score<M> sc(a, h);
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
+
+  const int tiles = (a.S + kTile - 1) / kTile;
+  for (int base = 0; base < tiles; base += kList) {
+    const int count =
+        list_tiles<true, OWN>(a, n, own0, base, sm.list, &sm.count);
+    s16x8 kr[L::kPer], vr[L::kPer];
+    int dr = -1;
+    unsigned rows = 0;
+    auto fetch = [&](int e) {
+      const int t0 =
+          (__builtin_amdgcn_readfirstlane(sm.list[e]) >> 1) * kTile;
+      ks.load(t0, a.S, kr);
+      vs.load(t0, a.S, vr);
+      rows = live_rows<DP>(doc, t0, a.S);
+      if (threadIdx.x < kTile) dr = doc_of(a, n, t0 + threadIdx.x);
+    };
+    auto keep = [&](int buf) {
+      Stream<DP>::store(sm.tile[buf][0], rows, a.D, kr);
+      Stream<DP>::store(sm.tile[buf][1], rows, a.D, vr);
+      if (threadIdx.x < kTile) sm.doc[buf][threadIdx.x] = dr;
+    };
+    if (count > 0) {
+      fetch(0);
+      keep(0);
+      __syncthreads();
+    }
+    for (int e = 0; e < count; ++e) {
+      const int buf = e & 1;
+      const bool more = e + 1 < count;
+      const int entry = __builtin_amdgcn_readfirstlane(sm.list[e]);
+      if (more) fetch(e + 1);
+      const int t0 = (entry >> 1) * kTile;
+#pragma unroll
+      for (int i = 0; i < KB; ++i) {
+        const int kb = KS == 1 ? i : part;
+        const char* kt = sm.tile[buf][0] + kb * (L::kBytes / 2);
+        const char* vt = sm.tile[buf][1] + kb * (L::kBytes / 2);
+        const int other = kb * 32 + 4 * half;
+        f32x16 z = 0.f, dp = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          z = mfma<T>(L::rows(kt, kk), qf[kk], z);
+          dp = mfma<T>(L::rows(vt, kk), gf[kk], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] -= delta;
+        if constexpr (M == kCap) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float th = fast_tanh(z[r] * sc.cap_in);
+            dp[r] *= 1.f - th * th;
+          }
+        }
+        sc.shape(z, static_cast<float>(own - t0 - other));
+        if (!(entry & 1))
+          mask<true>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          dp[r] *= fast_exp2(__builtin_fmaf(z[r], sc.c, -lse));
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const s16x8 x = round8<T>(dp, s);
+#pragma unroll
+          for (int db = 0; db < DP / 32; ++db)
+            acc[db] = mfma<T>(L::cols(kt, s, db), x, acc[db]);
+        }
+      }
+      if (more) keep(buf ^ 1);
+      __syncthreads();
+    }
+  }
+  if constexpr (KS == 2) {
+    float* at = reinterpret_cast<float*>(&sm.tile[0][0][0]) +
+                (wave / 2) * (DP / 2) * kWave;
+    __syncthreads();
+    if (part == 1) leave(at, acc);
+    __syncthreads();
+    if (part == 1) return;
+    f32x16 o[DP / 32];
+    pick_up(at, o);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] += o[i];
+  }
+  if (own < a.S)
+    store_cols<T, DP>(static_cast<T*>(a.gq.p) + n * a.gq.sn + own * a.gq.ss +
+                          h * a.gq.sh,
+                      acc, a.scale, live, a.D);
+}
+
+template <typename T, int DP, Mode M, int KS>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void
+masked_attn_dkv_kernel(MaskedAttn a) {
+  using L = Tile<DP>;
+  constexpr int OWN = 128 / KS, KB = 2 / KS;
+  __shared__ __align__(16) Smem<DP> sm;
+  int n, hk, own0;
+  locate<OWN>(a, a.Hkv, false, &n, &hk, &own0);
+  const int group = a.H / a.Hkv;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
+  const int own = own0 + (wave / KS) * 32 + (lane & 31);
+  const int found = doc_of(a, n, own);
+  const bool live = found >= 0;
+  const int own_doc = live ? found : -2;
+  const int lim = pair_limit<false>(a, n, own);
+  const int* doc =
+      a.doc != nullptr ? a.doc + static_cast<int64_t>(n) * a.S : nullptr;
+  s16x8 kf[DP / 16], vf[DP / 16];
+  own_rows<DP>(row_of(a.k, n, hk) + own * a.k.ss, live, a.D, kf);
+  own_rows<DP>(row_of(a.v, n, hk) + own * a.v.ss, live, a.D, vf);
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = 0.f;
+
+  const int tiles = (a.S + kTile - 1) / kTile;
+  for (int base = 0; base < tiles; base += kList) {
+    const int count =
+        list_tiles<false, OWN>(a, n, own0, base, sm.list, &sm.count);
+    // every head of the group over the same list, one after another
+    for (int hi = 0; hi < group && count > 0; ++hi) {
+      const int h = hk * group + hi;
+      const Score<M> sc(a, h);
+      const Stream<DP> qs(row_of(a.q, n, h), a.q.ss, a.D);
+      const Stream<DP> gs(row_of(a.go, n, h), a.go.ss, a.D);
+      const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S;
+      s16x8 qr[L::kPer], gr[L::kPer];
+      int dr = -1;
+      float lr = INFINITY, er = 0.f;
+      unsigned rows = 0;
+      auto fetch = [&](int e) {
+        const int t0 =
+          (__builtin_amdgcn_readfirstlane(sm.list[e]) >> 1) * kTile;
+        qs.load(t0, a.S, qr);
+        gs.load(t0, a.S, gr);
+        rows = live_rows<DP>(doc, t0, a.S);
+        if (threadIdx.x < kTile) {
+          const int tok = t0 + threadIdx.x;
+          dr = doc_of(a, n, tok);
+          lr = tok < a.S ? a.lse[stat + tok] : INFINITY;
+          er = tok < a.S ? a.delta[stat + tok] : 0.f;
+        }
+      };
+      auto keep = [&](int buf) {
+        Stream<DP>::store(sm.tile[buf][0], rows, a.D, qr);
+        Stream<DP>::store(sm.tile[buf][1], rows, a.D, gr);
+        if (threadIdx.x < kTile) {
+          sm.doc[buf][threadIdx.x] = dr;
+          sm.lse[buf][threadIdx.x] = lr;
+          sm.delta[buf][threadIdx.x] = er;
+        }
+      };
+      fetch(0);
+      keep(0);
+      __syncthreads();
+      for (int e = 0; e < count; ++e) {
+        const int buf = e & 1;
+        const bool more = e + 1 < count;
+        const int entry = __builtin_amdgcn_readfirstlane(sm.list[e]);
+        if (more) fetch(e + 1);
+        const int t0 = (entry >> 1) * kTile;
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+          const int qb = KS == 1 ? i : part;
+          const char* qt = sm.tile[buf][0] + qb * (L::kBytes / 2);
+          const char* gt = sm.tile[buf][1] + qb * (L::kBytes / 2);
+          const int other = qb * 32 + 4 * half;
+          f32x16 z = 0.f, dp = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            z = mfma<T>(L::rows(qt, kk), kf[kk], z);
+            dp = mfma<T>(L::rows(gt, kk), vf[kk], dp);
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 de = *reinterpret_cast<const float4*>(
+                sm.delta[buf] + other + g * 8);
+            dp[g * 4] -= de.x;
+            dp[g * 4 + 1] -= de.y;
+            dp[g * 4 + 2] -= de.z;
+            dp[g * 4 + 3] -= de.w;
+          }
+          if constexpr (M == kCap) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float th = fast_tanh(z[r] * sc.cap_in);
+              dp[r] *= 1.f - th * th;
+            }
+          }
+          sc.shape(z, static_cast<float>(own - t0 - other));
+          if (!(entry & 1))
+            mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 ls = *reinterpret_cast<const float4*>(
+                sm.lse[buf] + other + g * 8);
+            const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int r = g * 4 + j;
+              z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -l4[j]));
+              dp[r] *= z[r];
+              z[r] *= kLift<T>;
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const s16x8 p = round8<T>(z, s);
+            const s16x8 x = round8<T>(dp, s);
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) {
+              dv[db] = mfma<T>(L::cols(gt, s, db), p, dv[db]);
+              dk[db] = mfma<T>(L::cols(qt, s, db), x, dk[db]);
+            }
+          }
+        }
+        if (more) keep(buf ^ 1);
+        __syncthreads();
+      }
+    }
+  }
+  if constexpr (KS == 2) {
+    float* at = reinterpret_cast<float*>(&sm.tile[0][0][0]) +
+                (wave / 2) * DP * kWave;
+    __syncthreads();
+    if (part == 1) {
+      leave(at, dk);
+      leave(at + (DP / 2) * kWave, dv);
+    }
+    __syncthreads();
+    if (part == 1) return;
+    f32x16 o[DP / 32];
+    pick_up(at, o);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) dk[i] += o[i];
+    pick_up(at + (DP / 2) * kWave, o);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) dv[i] += o[i];
+  }
+  if (own < a.S) {
+    store_cols<T, DP>(static_cast<T*>(a.gk.p) + n * a.gk.sn + own * a.gk.ss +
+                          hk * a.gk.sh,
+                      dk, a.scale, live, a.D);
+    store_cols<T, DP>(static_cast<T*>(a.gv.p) + n * a.gv.sn + own * a.gv.ss +
+                          hk * a.gv.sh,
+                      dv, 1.f / kLift<T>, live, a.D);
+  }
+}
+
+struct Backward {
+  const MaskedAttn& a;
+  hipStream_t stream;
+
+  template <typename T, int DP, Mode M>
+  void run() const {
+    if (masked_attn_split(a, a.H))
+      masked_attn_dq_kernel<T, DP, M, 2>
+          <<<a.N * a.H * ((a.S + 63) / 64), 256, 0, stream>>>(a);
+    else
+      masked_attn_dq_kernel<T, DP, M, 1>
+          <<<a.N * a.H * ((a.S + 127) / 128), 256, 0, stream>>>(a);
+    if (masked_attn_split(a, a.Hkv))
+      masked_attn_dkv_kernel<T, DP, M, 2>
+          <<<a.N * a.Hkv * ((a.S + 63) / 64), 256, 0, stream>>>(a);
+    else
+      masked_attn_dkv_kernel<T, DP, M, 1>
+          <<<a.N * a.Hkv * ((a.S + 127) / 128), 256, 0, stream>>>(a);
+  }
+};
+
+}  // namespace
+
+void launch_masked_attn_bwd(const MaskedAttn& a, Elem type,
+                            hipStream_t stream) {
+  with_type(Backward{a, stream}, a, type);
+}
+
+}  // namespace colearn

@@ -29,7 +29,8 @@ ext = CUDAExtension(
         os.path.join(CSRC, "bindings_encoder.cpp"),
         os.path.join(CSRC, "adamw.hip"),
         os.path.join(CSRC, "add_norm.hip"),
-        os.path.join(CSRC, "masked_attn.hip"),
+        os.path.join(CSRC, "masked_attn_fwd.hip"),
+        os.path.join(CSRC, "masked_attn_bwd.hip"),
         os.path.join(CSRC, "fused_optim.hip"),
         os.path.join(CSRC, "dp_topk.hip"),
         os.path.join(CSRC, "norms.hip"),
