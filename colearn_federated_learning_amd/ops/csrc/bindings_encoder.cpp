@@ -304,7 +304,7 @@ torch::Tensor readable(const torch::Tensor& t) {
   bool ok = t.stride(3) == 1 && aligned16(t);
   for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
   // a tile's rows are addressed with 32 bits
-  ok = ok && t.stride(1) >= 0 && t.stride(1) <= (1 << 24);
+  ok = ok && t.stride(1) >= 0 && t.stride(1) <= (1 << 23);
   return ok ? t : t.contiguous();
 }
 
@@ -336,9 +336,9 @@ MaskedAttn describe(const torch::Tensor& q, const torch::Tensor& k,
   TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0,
               "masked_attn: head sizes are multiples of 8 up to 128, not ", D);
   constexpr int64_t kMost = std::numeric_limits<int>::max();
-  TORCH_CHECK(S <= kMost - 256 && N <= kMost &&
+  TORCH_CHECK(S <= (1 << 22) && N <= kMost &&
                   N * H * ((S + 63) / 64) <= kMost,
-              "masked_attn: too many tokens");
+              "masked_attn: too many tokens (a sequence has at most 2^22)");
   TORCH_CHECK(scale > 0.0 && softcap >= 0.0,
               "masked_attn: the scale must be positive, the cap not negative");
   MaskedAttn a{};
@@ -386,10 +386,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> masked_attn_fwd(
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   auto o = torch::empty({a.N, a.S, a.H, a.D}, q.options());
   auto lse = torch::empty({a.N, a.H, a.S}, q.options().dtype(torch::kFloat32));
-  // A summary costs a launch; up to four tiles a row testing every pair is
-  // cheaper.
-  const int64_t tiles = (a.S + kAttnTile - 1) / kAttnTile;
-  const bool summary = doc.has_value() && tiles > 4;
+  const int64_t tiles = (a.S + kAttnGroup - 1) / kAttnGroup;
+  const bool summary = doc.has_value() && a.S > kAttnShort;
   auto sum = torch::empty({summary ? a.N * tiles : 0, 4},
                           q.options().dtype(torch::kInt32));
   if (o.numel() == 0) return {o, lse, sum};
@@ -428,13 +426,14 @@ void masked_attn_bwd(torch::Tensor go, torch::Tensor q, torch::Tensor k,
   check_like(gv, v, "masked_attn: v's gradient");
   check_gpu(lse, q.device(), "masked_attn: row statistics");
   check_gpu(sum, q.device(), "masked_attn: summary");
-  const int64_t tiles = (a.S + kAttnTile - 1) / kAttnTile;
+  const int64_t tiles = (a.S + kAttnGroup - 1) / kAttnGroup;
+  const int64_t entries =
+      doc.has_value() && a.S > kAttnShort ? a.N * tiles * 4 : 0;
   TORCH_CHECK(lse.scalar_type() == torch::kFloat32 && lse.is_contiguous() &&
                   lse.numel() == static_cast<int64_t>(a.N) * a.H * a.S,
               "masked_attn: row statistics do not match");
   TORCH_CHECK(sum.scalar_type() == torch::kInt32 && sum.is_contiguous() &&
-                  (sum.numel() == 0 ||
-                   (doc.has_value() && sum.numel() == a.N * tiles * 4)),
+                  sum.numel() == entries,
               "masked_attn: the summary does not match");
   for (const auto& t : {gq, gk, gv}) {
     bool ok = t.stride(3) == 1 && aligned16(t);

@@ -82,7 +82,9 @@ void launch_add_norm_bwd(const AddNormBwd& b, Elem type, bool vec,
                          hipStream_t stream);
 
 // ---- masked attention ---------------------------------------------------------
-constexpr int kAttnTile = 64;  // tokens a tile of the mask's summary
+constexpr int kAttnTile = 64;     // streamed tokens a tile
+constexpr int kAttnGroup = 32;    // tokens an entry of the mask's summary
+constexpr int kAttnShort = 1024;  // up to here workgroups make their own
 
 struct HeadView {  // [N, S, heads, D] with D contiguous
   void* p;
@@ -95,7 +97,7 @@ struct MaskedAttn {
   const int* doc;             // [N, S], or null
   const int* prefix;          // [N], or null
   const float* slopes;        // [H], or null
-  int4* tiles;                // [N, ceil(S / 64)] summary of doc, or null
+  int4* tiles;                // [N, ceil(S / 32)] summary of doc, or null
   float* lse;                 // [N, H, S], base 2; +inf for empty rows
   float* delta;               // [N, H, S], backward only
   int N, S, H, Hkv, D;

@@ -10,7 +10,7 @@ using namespace masked_attn;
 namespace {
 
 template <typename T, int DP, Mode M, int KS>
-__global__ __launch_bounds__(256, 2) void masked_attn_dq_kernel(
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
     MaskedAttn a) {
   using L = Tile<DP>;
   constexpr int OWN = 128 / KS, KB = 2 / KS;
@@ -18,15 +18,16 @@ __global__ __launch_bounds__(256, 2) void masked_attn_dq_kernel(
   int n, h, own0;
   locate<OWN>(a, a.H, a.causal, &n, &h, &own0);
   const int hk = h / (a.H / a.Hkv);
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
   const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
   const int own = own0 + (wave / KS) * 32 + (lane & 31);
   const int found = doc_of(a, n, own);
   const bool live = found >= 0;
   const int own_doc = live ? found : -2;
   const int lim = pair_limit<true>(a, n, own);
-  const int* doc =
-      a.doc != nullptr ? a.doc + static_cast<int64_t>(n) * a.S : nullptr;
+  Docs docs(a, n);
+  const int4* sum = summary_of(a, n, sm.sum);
   const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss, a.D);
   const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss, a.D);
   s16x8 qf[DP / 16], gf[DP / 16];
@@ -59,38 +60,40 @@ __global__ __launch_bounds__(256, 2) void masked_attn_dq_kernel(
 
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
-    const int count =
-        list_tiles<true, OWN>(a, n, own0, base, sm.list, &sm.count);
+    const int count = list_tiles<true, OWN / 32>(a, n, own0, base, sum,
+                                                 sm.list, &sm.count);
+    if (count == 0) continue;
     s16x8 kr[L::kPer], vr[L::kPer];
-    int dr = -1;
-    unsigned rows = 0;
-    auto fetch = [&](int e) {
-      const int t0 =
-          (__builtin_amdgcn_readfirstlane(sm.list[e]) >> 1) * kTile;
+    auto fetch = [&](unsigned entry) {
+      const int t0 = first_of(entry);
       ks.load(t0, a.S, kr);
       vs.load(t0, a.S, vr);
-      rows = live_rows<DP>(doc, t0, a.S);
-      if (threadIdx.x < kTile) dr = doc_of(a, n, t0 + threadIdx.x);
+      docs.load(t0, a.S);
     };
-    auto keep = [&](int buf) {
-      Stream<DP>::store(sm.tile[buf][0], rows, a.D, kr);
-      Stream<DP>::store(sm.tile[buf][1], rows, a.D, vr);
-      if (threadIdx.x < kTile) sm.doc[buf][threadIdx.x] = dr;
+    auto keep = [&](int buf, unsigned entry) {
+      const int t0 = first_of(entry);
+      const bool some = ragged(entry, a.S) || a.D < DP;
+      const unsigned long long live = docs.live(t0, a.S);
+      Stream<DP>::store(sm.tile[buf][0], some, live, a.D, kr);
+      Stream<DP>::store(sm.tile[buf][1], some, live, a.D, vr);
+      if (threadIdx.x < kTile) sm.doc[buf][threadIdx.x] = docs.own(t0, a.S);
     };
-    if (count > 0) {
-      fetch(0);
-      keep(0);
-      __syncthreads();
-    }
+    unsigned entry = entry_of(sm.list, 0, count);
+    unsigned next = entry_of(sm.list, 1, count);
+    fetch(entry);
+    keep(0, entry);
+    __syncthreads();
     for (int e = 0; e < count; ++e) {
       const int buf = e & 1;
-      const bool more = e + 1 < count;
-      const int entry = __builtin_amdgcn_readfirstlane(sm.list[e]);
-      if (more) fetch(e + 1);
-      const int t0 = (entry >> 1) * kTile;
+      if (e + 1 < count) fetch(next);
+      const unsigned after = sm.list[min(e + 2, count - 1)];
+      const int t0 = first_of(entry);
+      const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
 #pragma unroll
       for (int i = 0; i < KB; ++i) {
         const int kb = KS == 1 ? i : part;
+        const unsigned c = (cls >> (2 * kb)) & 3;
+        if (c == 0) continue;
         const char* kt = sm.tile[buf][0] + kb * (L::kBytes / 2);
         const char* vt = sm.tile[buf][1] + kb * (L::kBytes / 2);
         const int other = kb * 32 + 4 * half;
@@ -110,7 +113,7 @@ __global__ __launch_bounds__(256, 2) void masked_attn_dq_kernel(
           }
         }
         sc.shape(z, static_cast<float>(own - t0 - other));
-        if (!(entry & 1))
+        if (c == 1)
           mask<true>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -123,7 +126,9 @@ __global__ __launch_bounds__(256, 2) void masked_attn_dq_kernel(
             acc[db] = mfma<T>(L::cols(kt, s, db), x, acc[db]);
         }
       }
-      if (more) keep(buf ^ 1);
+      if (e + 1 < count) keep(buf ^ 1, next);
+      entry = next;
+      next = __builtin_amdgcn_readfirstlane(after);
       __syncthreads();
     }
   }
@@ -154,15 +159,16 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   int n, hk, own0;
   locate<OWN>(a, a.Hkv, false, &n, &hk, &own0);
   const int group = a.H / a.Hkv;
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
   const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
   const int own = own0 + (wave / KS) * 32 + (lane & 31);
   const int found = doc_of(a, n, own);
   const bool live = found >= 0;
   const int own_doc = live ? found : -2;
   const int lim = pair_limit<false>(a, n, own);
-  const int* doc =
-      a.doc != nullptr ? a.doc + static_cast<int64_t>(n) * a.S : nullptr;
+  Docs docs(a, n);
+  const int4* sum = summary_of(a, n, sm.sum);
   s16x8 kf[DP / 16], vf[DP / 16];
   own_rows<DP>(row_of(a.k, n, hk) + own * a.k.ss, live, a.D, kf);
   own_rows<DP>(row_of(a.v, n, hk) + own * a.v.ss, live, a.D, vf);
@@ -172,8 +178,8 @@ masked_attn_dkv_kernel(MaskedAttn a) {
 
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
-    const int count =
-        list_tiles<false, OWN>(a, n, own0, base, sm.list, &sm.count);
+    const int count = list_tiles<false, OWN / 32>(a, n, own0, base, sum,
+                                                  sm.list, &sm.count);
     // every head of the group over the same list, one after another
     for (int hi = 0; hi < group && count > 0; ++hi) {
       const int h = hk * group + hi;
@@ -182,43 +188,46 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       const Stream<DP> gs(row_of(a.go, n, h), a.go.ss, a.D);
       const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S;
       s16x8 qr[L::kPer], gr[L::kPer];
-      int dr = -1;
-      float lr = INFINITY, er = 0.f;
-      unsigned rows = 0;
-      auto fetch = [&](int e) {
-        const int t0 =
-          (__builtin_amdgcn_readfirstlane(sm.list[e]) >> 1) * kTile;
+      float lr, er;
+      auto fetch = [&](unsigned entry) {
+        const int t0 = first_of(entry);
         qs.load(t0, a.S, qr);
         gs.load(t0, a.S, gr);
-        rows = live_rows<DP>(doc, t0, a.S);
+        docs.load(t0, a.S);
+        const int tok =
+            min(t0 + static_cast<int>(threadIdx.x) % kTile, a.S - 1);
+        lr = a.lse[stat + tok];
+        er = a.delta[stat + tok];
+      };
+      auto keep = [&](int buf, unsigned entry) {
+        const int t0 = first_of(entry);
+        const bool some = ragged(entry, a.S) || a.D < DP;
+        const unsigned long long live = docs.live(t0, a.S);
+        Stream<DP>::store(sm.tile[buf][0], some, live, a.D, qr);
+        Stream<DP>::store(sm.tile[buf][1], some, live, a.D, gr);
         if (threadIdx.x < kTile) {
-          const int tok = t0 + threadIdx.x;
-          dr = doc_of(a, n, tok);
-          lr = tok < a.S ? a.lse[stat + tok] : INFINITY;
-          er = tok < a.S ? a.delta[stat + tok] : 0.f;
+          const bool past = t0 + static_cast<int>(threadIdx.x) >= a.S;
+          sm.doc[buf][threadIdx.x] = docs.own(t0, a.S);
+          sm.lse[buf][threadIdx.x] = past ? INFINITY : lr;
+          sm.delta[buf][threadIdx.x] = past ? 0.f : er;
         }
       };
-      auto keep = [&](int buf) {
-        Stream<DP>::store(sm.tile[buf][0], rows, a.D, qr);
-        Stream<DP>::store(sm.tile[buf][1], rows, a.D, gr);
-        if (threadIdx.x < kTile) {
-          sm.doc[buf][threadIdx.x] = dr;
-          sm.lse[buf][threadIdx.x] = lr;
-          sm.delta[buf][threadIdx.x] = er;
-        }
-      };
-      fetch(0);
-      keep(0);
+      unsigned entry = entry_of(sm.list, 0, count);
+      unsigned next = entry_of(sm.list, 1, count);
+      fetch(entry);
+      keep(0, entry);
       __syncthreads();
       for (int e = 0; e < count; ++e) {
         const int buf = e & 1;
-        const bool more = e + 1 < count;
-        const int entry = __builtin_amdgcn_readfirstlane(sm.list[e]);
-        if (more) fetch(e + 1);
-        const int t0 = (entry >> 1) * kTile;
+        if (e + 1 < count) fetch(next);
+        const unsigned after = sm.list[min(e + 2, count - 1)];
+        const int t0 = first_of(entry);
+        const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
 #pragma unroll
         for (int i = 0; i < KB; ++i) {
           const int qb = KS == 1 ? i : part;
+          const unsigned c = (cls >> (2 * qb)) & 3;
+          if (c == 0) continue;
           const char* qt = sm.tile[buf][0] + qb * (L::kBytes / 2);
           const char* gt = sm.tile[buf][1] + qb * (L::kBytes / 2);
           const int other = qb * 32 + 4 * half;
@@ -245,7 +254,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
             }
           }
           sc.shape(z, static_cast<float>(own - t0 - other));
-          if (!(entry & 1))
+          if (c == 1)
             mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -271,7 +280,9 @@ masked_attn_dkv_kernel(MaskedAttn a) {
             }
           }
         }
-        if (more) keep(buf ^ 1);
+        if (e + 1 < count) keep(buf ^ 1, next);
+        entry = next;
+        next = __builtin_amdgcn_readfirstlane(after);
         __syncthreads();
       }
     }

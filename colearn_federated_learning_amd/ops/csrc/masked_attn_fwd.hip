@@ -9,42 +9,38 @@ using namespace masked_attn;
 
 namespace {
 
-// summary of one 64-token tile of doc: smallest and largest document, and
-// whether there is padding; (INT_MAX, -1) if there is nothing else
+// summaries of 32 tokens each, two a workgroup; groups: of a sequence
 __global__ __launch_bounds__(64) void masked_attn_tiles_kernel(
-    const int* __restrict__ doc, int4* __restrict__ tiles, int S, int count) {
-  const int n = blockIdx.x / count;  // count: tiles a sequence
-  const int tok = (blockIdx.x - n * count) * kTile + threadIdx.x;
-  const int d = tok < S ? doc[static_cast<int64_t>(n) * S + tok] : 0;
-  const bool real = tok < S && d >= 0;
-  int lo = real ? d : 0x7fffffff, hi = real ? d : -1;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    lo = min(lo, __shfl_xor(lo, off));
-    hi = max(hi, __shfl_xor(hi, off));
-  }
-  const bool pad = __any(tok < S && d < 0);
-  if (threadIdx.x == 0) tiles[blockIdx.x] = make_int4(lo, hi, pad, 0);
+    const int* __restrict__ doc, int4* __restrict__ tiles, int S,
+    int groups) {
+  const int pairs = (groups + 1) / 2;
+  const int n = blockIdx.x / pairs;
+  const int tok = (blockIdx.x - n * pairs) * 64 + threadIdx.x;
+  const int4 s = summarise(
+      doc[static_cast<int64_t>(n) * S + min(tok, S - 1)], tok < S);
+  if (threadIdx.x % 32 == 0 && tok < S)
+    tiles[static_cast<int64_t>(n) * groups + tok / 32] = s;
 }
 
 template <typename T, int DP, Mode M, int KS>
-__global__ __launch_bounds__(256, 2) void masked_attn_fwd_kernel(
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel(
     MaskedAttn a) {
   using L = Tile<DP>;
-  constexpr int OWN = 128 / KS, KB = 2 / KS;
+  constexpr int OWN = 128 / KS;
   __shared__ __align__(16) Smem<DP> sm;
   int n, h, own0;
   locate<OWN>(a, a.H, a.causal, &n, &h, &own0);
   const int hk = h / (a.H / a.Hkv);
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
   const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
   const int own = own0 + (wave / KS) * 32 + (lane & 31);
   const int found = doc_of(a, n, own);
   const bool live = found >= 0;
   const int own_doc = live ? found : -2;
   const int lim = pair_limit<true>(a, n, own);
-  const int* doc =
-      a.doc != nullptr ? a.doc + static_cast<int64_t>(n) * a.S : nullptr;
+  Docs docs(a, n);
+  const int4* sum = summary_of(a, n, sm.sum);
   const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss, a.D);
   const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss, a.D);
   s16x8 qf[DP / 16];
@@ -55,86 +51,91 @@ __global__ __launch_bounds__(256, 2) void masked_attn_fwd_kernel(
   for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
   float m = -INFINITY, l = 0.f;  // m: of c z; l: this half's share
 
+  // 32 streamed keys from t0 on; mixed: some pairs of them are not attended
+  auto work = [&](const char* kt, const char* vt, const int* dt, int t0,
+                  bool mixed) {
+    f32x16 z = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      z = mfma<T>(L::rows(kt, kk), qf[kk], z);
+    const int other = t0 + 4 * half;
+    sc.shape(z, static_cast<float>(own - other));
+    if (mixed) mask<true>(z, own_doc, lim, other, dt + 4 * half);
+    float mx = z[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, z[r]);
+    mx *= sc.c;
+    // The sums are kept relative to a maximum that may be outgrown by 2^8
+    // before they are scaled anew: p stays within both types' range, and its
+    // rounding is relative.
+    if (__any(mx > m + 8.f)) {
+      const float top = fmaxf(m, fmaxf(mx, other_half(mx)));
+      // a row that has met nothing yet stays at -inf without NaN
+      const float f = fast_exp2(m - (top == -INFINITY ? 0.f : top));
+      m = top;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
+    }
+    const float top = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -top));
+      l += z[r];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const s16x8 p = round8<T>(z, s);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+        acc[db] = mfma<T>(L::cols(vt, s, db), p, acc[db]);
+    }
+  };
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
-    const int count =
-        list_tiles<true, OWN>(a, n, own0, base, sm.list, &sm.count);
+    const int count = list_tiles<true, OWN / 32>(a, n, own0, base, sum,
+                                                 sm.list, &sm.count);
+    if (count == 0) continue;
     s16x8 kr[L::kPer], vr[L::kPer];
-    int dr = -1;
-    unsigned rows = 0;
-    auto fetch = [&](int e) {
-      const int t0 =
-          (__builtin_amdgcn_readfirstlane(sm.list[e]) >> 1) * kTile;
+    auto fetch = [&](unsigned entry) {
+      const int t0 = first_of(entry);
       ks.load(t0, a.S, kr);
       vs.load(t0, a.S, vr);
-      rows = live_rows<DP>(doc, t0, a.S);
-      if (threadIdx.x < kTile) dr = doc_of(a, n, t0 + threadIdx.x);
+      docs.load(t0, a.S);
     };
-    auto keep = [&](int buf) {
-      Stream<DP>::store(sm.tile[buf][0], rows, a.D, kr);
-      Stream<DP>::store(sm.tile[buf][1], rows, a.D, vr);
-      if (threadIdx.x < kTile) sm.doc[buf][threadIdx.x] = dr;
+    auto keep = [&](int buf, unsigned entry) {
+      const int t0 = first_of(entry);
+      const bool some = ragged(entry, a.S) || a.D < DP;
+      const unsigned long long live = docs.live(t0, a.S);
+      Stream<DP>::store(sm.tile[buf][0], some, live, a.D, kr);
+      Stream<DP>::store(sm.tile[buf][1], some, live, a.D, vr);
+      if (threadIdx.x < kTile) sm.doc[buf][threadIdx.x] = docs.own(t0, a.S);
     };
-    if (count > 0) {
-      fetch(0);
-      keep(0);
-      __syncthreads();
-    }
+    unsigned entry = entry_of(sm.list, 0, count);
+    unsigned next = entry_of(sm.list, 1, count);
+    fetch(entry);
+    keep(0, entry);
+    __syncthreads();
     for (int e = 0; e < count; ++e) {
       const int buf = e & 1;
-      const bool more = e + 1 < count;
-      const int entry = __builtin_amdgcn_readfirstlane(sm.list[e]);
-      if (more) fetch(e + 1);
-      const int t0 = (entry >> 1) * kTile;
-      f32x16 z[KB];
-      float mx = -INFINITY;
+      if (e + 1 < count) fetch(next);
+      const unsigned after = sm.list[min(e + 2, count - 1)];
+      const int t0 = first_of(entry);
+      const char* kt = sm.tile[buf][0];
+      const char* vt = sm.tile[buf][1];
+      const int* dt = sm.doc[buf];
+      const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
 #pragma unroll
-      for (int i = 0; i < KB; ++i) {
-        const int kb = KS == 1 ? i : part;
-        const char* kt = sm.tile[buf][0] + kb * (L::kBytes / 2);
-        z[i] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          z[i] = mfma<T>(L::rows(kt, kk), qf[kk], z[i]);
+      for (int i = 0; i < 2 / KS; ++i) {
+        const int hf = KS == 2 ? part : i;
+        const unsigned c = (cls >> (2 * hf)) & 3;
+        if (c != 0)
+          work(kt + hf * (L::kBytes / 2), vt + hf * (L::kBytes / 2),
+               dt + hf * 32, t0 + hf * 32, c == 1);
       }
-#pragma unroll
-      for (int i = 0; i < KB; ++i) {
-        const int other = (KS == 1 ? i : part) * 32 + 4 * half;
-        sc.shape(z[i], static_cast<float>(own - t0 - other));
-        if (!(entry & 1))
-          mask<true>(z[i], own_doc, lim, t0 + other, sm.doc[buf] + other);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, z[i][r]);
-      }
-      mx = fmaxf(mx, other_half(mx)) * sc.c;
-      if (__any(mx > m)) {
-        const float top = fmaxf(m, mx);
-        // a row that has met nothing yet stays at -inf without NaN
-        const float f = fast_exp2(m - (top == -INFINITY ? 0.f : top));
-        m = top;
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
-      }
-      const float top = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int i = 0; i < KB; ++i) {
-        const int kb = KS == 1 ? i : part;
-        const char* vt = sm.tile[buf][1] + kb * (L::kBytes / 2);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          z[i][r] = fast_exp2(__builtin_fmaf(z[i][r], sc.c, -top));
-          l += z[i][r];
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const s16x8 p = round8<T>(z[i], s);
-#pragma unroll
-          for (int db = 0; db < DP / 32; ++db)
-            acc[db] = mfma<T>(L::cols(vt, s, db), p, acc[db]);
-        }
-      }
-      if (more) keep(buf ^ 1);
+      if (e + 1 < count) keep(buf ^ 1, next);
+      entry = next;
+      next = __builtin_amdgcn_readfirstlane(after);
       __syncthreads();
     }
   }
@@ -199,9 +200,9 @@ bool masked_attn_split(const MaskedAttn& a, int heads) {
 }
 
 void launch_masked_attn_tiles(const MaskedAttn& a, hipStream_t stream) {
-  const int tiles = (a.S + kTile - 1) / kTile;
-  masked_attn_tiles_kernel<<<tiles * a.N, 64, 0, stream>>>(a.doc, a.tiles,
-                                                           a.S, tiles);
+  const int groups = (a.S + 31) / 32;
+  masked_attn_tiles_kernel<<<(groups + 1) / 2 * a.N, 64, 0, stream>>>(
+      a.doc, a.tiles, a.S, groups);
 }
 
 void launch_masked_attn_fwd(const MaskedAttn& a, Elem type,

@@ -36,10 +36,11 @@
 // fp32.  Probabilities and dz are rounded to the operands' type for the second
 // products; the sums in the denominator are of the unrounded ones.
 //
-// The mask is summarised per 64 tokens (smallest and largest document, any
-// padding).  A workgroup first lists the tiles that it has to visit, each
-// marked whole (every pair attended: no test in the loop) or mixed; tiles
-// between documents that do not meet cost nothing.  Rows of padding are
+// The mask is summarised per 32 tokens (smallest and largest document, any
+// padding).  A workgroup first lists the tiles that it has to visit, with a
+// mark for every 32 x 32 pairs: none attended (the wave skips them), all (no
+// test in the loop) or some; tiles between documents that do not meet cost
+// nothing.  Rows of padding are
 // staged as zeros and rows of padding are written as zeros, so that whatever
 // a padded token holds reaches no result.
 //
@@ -60,6 +61,7 @@ namespace masked_attn {
 
 constexpr int kTile = kAttnTile;   // streamed tokens a tile
 constexpr int kList = 1024;        // tiles listed at a time
+constexpr int kShort = kAttnShort;  // tokens summarised by the workgroup itself
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What happens to a score before the exponential, besides its scale
@@ -151,68 +153,86 @@ struct Tile {
 };
 
 // One streamed operand [S, D]: this thread's 16 bytes of a tile's rows
-// threadIdx.x / kSlots + i kStep.  The row's offset in a tile is 32 bits (the
-// host sees to it), the tile's own 64.
+// threadIdx.x / kSlots + i kStep.  A row's offset in a tile is 32 bits of bytes
+// (the host sees to it), the tile's own 64.  Nothing here branches around a
+// load: loads behind a branch would be waited for where the paths meet, before
+// the tile at hand is worked on.
 template <int DP>
 struct Stream {
   using L = Tile<DP>;
   const short* base;
   int64_t ss;
-  unsigned off;
+  unsigned off, col;
 
   DEV_INLINE Stream(const short* p, int64_t stride, int D)
       : base(p), ss(stride) {
     const int slot = threadIdx.x % L::kSlots;
-    off = (threadIdx.x / L::kSlots) * static_cast<unsigned>(stride) +
-          (slot * 8 < D ? slot * 8 : 0);
+    col = slot * 8 < D ? slot * 16 : 0;
+    off = (threadIdx.x / L::kSlots) * static_cast<unsigned>(2 * stride) + col;
   }
+  // rows past S: the last one, which `store` leaves out
   DEV_INLINE void load(int t0, int S, s16x8 (&r)[L::kPer]) const {
-    const short* p = base + t0 * ss;
-    if (t0 + kTile <= S) {
+    const char* p = reinterpret_cast<const char*>(base + t0 * ss);
+    const unsigned row = static_cast<unsigned>(2 * ss);
+    unsigned at[L::kPer];
+#pragma unroll
+    for (int i = 0; i < L::kPer; ++i) at[i] = off + i * L::kStep * row;
+    if (t0 + kTile > S) {
 #pragma unroll
       for (int i = 0; i < L::kPer; ++i)
-        r[i] = *reinterpret_cast<const s16x8*>(p + i * (L::kStep * ss) + off);
-    } else {
+        at[i] = static_cast<unsigned>(min(
+                    static_cast<int>(threadIdx.x) / L::kSlots + i * L::kStep,
+                    S - 1 - t0)) * row + col;
+    }
+#pragma unroll
+    for (int i = 0; i < L::kPer; ++i)
+      r[i] = *reinterpret_cast<const s16x8*>(p + at[i]);
+  }
+  // Into LDS.  some: rows that `live` has no bit of, and columns past D, become
+  // zeros.
+  DEV_INLINE static void store(char* lds, bool some, unsigned long long live,
+                               int D, const s16x8 (&r)[L::kPer]) {
+    const int row = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
+    if (some) {
 #pragma unroll
       for (int i = 0; i < L::kPer; ++i) {
         const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-        r[i] = zero;
-        if (t0 + i * L::kStep + static_cast<int>(threadIdx.x) / L::kSlots < S)
-          r[i] =
-              *reinterpret_cast<const s16x8*>(p + i * (L::kStep * ss) + off);
+        const bool keep =
+            slot * 8 < D && ((live >> (row + i * L::kStep)) & 1);
+        *reinterpret_cast<s16x8*>(lds + L::at(row + i * L::kStep, slot)) =
+            keep ? r[i] : zero;
       }
-    }
-  }
-  // rows of padding and columns past D as zeros; live: bit i for pass i
-  DEV_INLINE static void store(char* lds, unsigned live, int D,
-                               const s16x8 (&r)[L::kPer]) {
-    const int row = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
-    const unsigned keep = slot * 8 < D ? live : 0;
+    } else {
 #pragma unroll
-    for (int i = 0; i < L::kPer; ++i) {
-      const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-      *reinterpret_cast<s16x8*>(lds + L::at(row + i * L::kStep, slot)) =
-          (keep >> i) & 1 ? r[i] : zero;
+      for (int i = 0; i < L::kPer; ++i)
+        *reinterpret_cast<s16x8*>(lds + L::at(row + i * L::kStep, slot)) =
+            r[i];
     }
   }
 };
 
-// documents of the rows that this thread stages: bit i set if row i is no
-// padding (rows past S are zeros already)
-template <int DP>
-DEV_INLINE unsigned live_rows(const int* doc, int t0, int S) {
-  using L = Tile<DP>;
-  if (doc == nullptr) return ~0u;
-  unsigned live = 0;
-#pragma unroll
-  for (int i = 0; i < L::kPer; ++i) {
-    const int tok =
-        min(t0 + i * L::kStep + static_cast<int>(threadIdx.x) / L::kSlots,
-            S - 1);
-    live |= (doc[tok] >= 0 ? 1u : 0u) << i;
+// The streamed tokens' documents: every wave's lanes hold those of the tile's
+// 64 tokens.
+struct Docs {
+  const int* doc;  // of this sequence, or null
+  int tok = 0;
+
+  DEV_INLINE Docs(const MaskedAttn& a, int n)
+      : doc(a.doc != nullptr ? a.doc + static_cast<int64_t>(n) * a.S
+                             : nullptr) {}
+  DEV_INLINE void load(int t0, int S) {
+    if (doc != nullptr)
+      tok = doc[min(t0 + static_cast<int>(threadIdx.x) % kTile, S - 1)];
   }
-  return live;
-}
+  // -1 for padding and past the end, 0 without documents
+  DEV_INLINE int own(int t0, int S) const {
+    return t0 + static_cast<int>(threadIdx.x) % kTile < S ? max(tok, -1) : -1;
+  }
+  // a bit for every token of the tile that is neither
+  DEV_INLINE unsigned long long live(int t0, int S) const {
+    return __ballot(own(t0, S) >= 0);
+  }
+};
 
 // right operand of an owned token's row: columns 16 kk + 8 h + 0..7
 template <int DP>
@@ -247,10 +267,11 @@ DEV_INLINE void store_cols(T* row, const f32x16 (&acc)[DP / 32], float f,
 }
 
 // What the pairs of tokens [q0, q1) x [k0, k1) are: 0 none attended, 1 some,
-// 2 all.  A tile that reaches past S counts as mixed on the key side only:
-// no query row past S is ever written, or has a statistic but +inf.
+// 2 all.  Keys past S count as not attended; queries past S are never written,
+// or have a statistic of +inf.
 DEV_INLINE int meet(bool causal, int prefix, int S, int q0, int q1, int k0,
                     int k1, bool doc, int4 a, int4 b) {
+  if (k0 >= S || q0 >= S) return 0;
   int c = k1 > S ? 1 : 2;
   const int qe = min(q1, S) - 1, ke = min(k1, S) - 1;
   if (causal) {
@@ -264,55 +285,98 @@ DEV_INLINE int meet(bool causal, int prefix, int S, int q0, int q1, int k0,
   return c;
 }
 
-DEV_INLINE int4 join(int4 a, int4 b) {
-  return make_int4(min(a.x, b.x), max(a.y, b.y), a.z | b.z, 0);
+// Summary of 32 tokens' documents (of the 32 lanes around this one): smallest,
+// largest, whether there is padding; (INT_MAX, -1) if there is nothing else.
+DEV_INLINE int4 summarise(int d, bool there) {
+  const bool real = there && d >= 0;
+  int lo = real ? d : 0x7fffffff, hi = real ? d : -1;
+  int pad = there && d < 0;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    lo = min(lo, __shfl_xor(lo, off));
+    hi = max(hi, __shfl_xor(hi, off));
+    pad |= __shfl_xor(pad, off);
+  }
+  return make_int4(lo, hi, pad, 0);
+}
+
+// The summary of a sequence: made before (a.tiles), or here in LDS for up to
+// kShort tokens, where a launch of its own would cost more.
+DEV_INLINE const int4* summary_of(const MaskedAttn& a, int n, int4* lds) {
+  if (a.doc == nullptr) return nullptr;
+  const int groups = (a.S + 31) / 32;
+  if (a.tiles != nullptr) return a.tiles + static_cast<int64_t>(n) * groups;
+  const int* doc = a.doc + static_cast<int64_t>(n) * a.S;
+  for (int t0 = 0; t0 < a.S; t0 += 256) {
+    const int t = t0 + threadIdx.x;
+    const int4 s = summarise(doc[min(t, a.S - 1)], t < a.S);
+    if (threadIdx.x % 32 == 0 && t < a.S) lds[t / 32] = s;
+  }
+  return lds;  // list_tiles begins with a barrier
 }
 
 // Lists the tiles of [base, base + kList) that meet the owned tokens from own0
-// on: (tile << 1) | whole, in order.  Called by the whole workgroup.
-template <bool OWN_Q, int OWN>
+// on, in order: tile << 16, and two bits (`meet`) for every 32 owned tokens g
+// and either half of the tile: bits 4 g + 2 half.  Called by the whole
+// workgroup.
+template <bool OWN_Q, int GROUPS>
 DEV_INLINE int list_tiles(const MaskedAttn& a, int n, int own0, int base,
-                          int* list, int* count) {
+                          const int4* sum, unsigned* list, int* count) {
   const int tiles = (a.S + kTile - 1) / kTile;
-  __syncthreads();  // the previous list is used up
+  __syncthreads();  // the summary is there, the previous list used up
   if (threadIdx.x < kWave) {
     const int lane = threadIdx.x;
     const int prefix = a.prefix != nullptr ? a.prefix[n] : 0;
-    const bool summary = a.tiles != nullptr;
-    const int4* row = a.tiles + static_cast<int64_t>(n) * tiles;
-    int4 mine = make_int4(0, 0, 0, 0);
-    if (summary) {
-      const int t = own0 / kTile;
-      mine = row[t];
-      if (OWN > kTile && t + 1 < tiles) mine = join(mine, row[t + 1]);
-    }
+    const int last = (a.S + 31) / 32 - 1;
+    const bool docs = sum != nullptr;
+    int4 mine[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+      mine[g] = docs ? sum[min(own0 / 32 + g, last)] : make_int4(0, 0, 0, 0);
     int found = 0;
     const int end = min(base + kList, tiles);
     for (int t0 = base; t0 < end; t0 += kWave) {
       const int t = t0 + lane;
-      int c = 0;
-      if (t < end) {
-        const int4 other = summary ? row[t] : mine;
-        const int s0 = t * kTile;
-        c = OWN_Q ? meet(a.causal, prefix, a.S, own0, own0 + OWN, s0,
-                         s0 + kTile, summary, mine, other)
-                  : meet(a.causal, prefix, a.S, s0, s0 + kTile, own0,
-                         own0 + OWN, summary, mine, other);
-        if (c == 2 && a.doc != nullptr && !summary) c = 1;
+      unsigned c = 0;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int4 other =
+            docs ? sum[min(t * 2 + hf, last)] : make_int4(0, 0, 0, 0);
+        const int s0 = t * kTile + hf * 32;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int o0 = own0 + g * 32;
+          const int x =
+              OWN_Q ? meet(a.causal, prefix, a.S, o0, o0 + 32, s0, s0 + 32,
+                           docs, mine[g], other)
+                    : meet(a.causal, prefix, a.S, s0, s0 + 32, o0, o0 + 32,
+                           docs, mine[g], other);
+          c |= x << (4 * g + 2 * hf);
+        }
       }
+      if (t >= end) c = 0;
       const unsigned long long hit = __ballot(c != 0);
       if (c != 0)
         list[found + __popcll(hit & ((1ull << lane) - 1))] =
-            (t << 1) | (c == 2);
+            (static_cast<unsigned>(t) << 16) | c;
       found += __popcll(hit);
     }
     if (lane == 0) *count = found;
   }
   __syncthreads();
-  return *count;
+  return __builtin_amdgcn_readfirstlane(*count);
 }
 
-// document of a streamed token: -1 for padding and past the end, 0 without
+DEV_INLINE unsigned entry_of(const unsigned* list, int e, int count) {
+  return __builtin_amdgcn_readfirstlane(list[min(e, count - 1)]);
+}
+DEV_INLINE int first_of(unsigned entry) { return (entry >> 16) * kTile; }
+// whether rows of a tile may have to be staged as zeros
+DEV_INLINE bool ragged(unsigned entry, int S) {
+  return (entry & 0x5555u) != 0 || first_of(entry) + kTile > S;
+}
+
+// document of an owned token: -1 for padding and past the end, 0 without
 // documents
 DEV_INLINE int doc_of(const MaskedAttn& a, int n, int tok) {
   if (tok >= a.S) return -1;
@@ -412,7 +476,8 @@ struct Smem {
   int doc[2][kTile];
   float lse[2][kTile];    // dk/dv only
   float delta[2][kTile];  // dk/dv only
-  int list[kList];
+  unsigned list[kList];
+  int4 sum[kShort / 32];
   int count;
 };
 
