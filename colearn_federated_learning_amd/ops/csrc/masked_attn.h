@@ -60,6 +60,7 @@ namespace masked_attn {
 constexpr int kTile = kAttnTile;   // streamed tokens a tile
 constexpr int kList = 1024;        // tiles listed at a time
 constexpr int kShort = kAttnShort;  // tokens summarised by the workgroup itself
+constexpr unsigned kZeros = 1u << 16;  // a list entry's mark
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What happens to a score before the exponential, besides its scale
@@ -70,6 +71,8 @@ typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
 
 template <typename T>
 DEV_INLINE f32x16 mfma(s16x8 a, s16x8 b, f32x16 c);
@@ -150,61 +153,49 @@ struct Tile {
   }
 };
 
-// One streamed operand [S, D]: this thread's 16 bytes of a tile's rows
-// threadIdx.x / kSlots + i kStep.  A row's offset in a tile is 32 bits of bytes
-// (the host sees to it), the tile's own 64.  Nothing here branches around a
-// load: loads behind a branch would be waited for where the paths meet, before
-// the tile at hand is worked on.
+// One streamed operand [S, D] on its way into LDS.  Each of a tile's kPer
+// passes moves 16 bytes a thread.  A row's offset in a tile is 32 bits of
+// bytes (the host sees to it), the tile's own 64.
 template <int DP>
 struct Stream {
   using L = Tile<DP>;
   const short* base;
   int64_t ss;
-  unsigned off, col;
 
-  DEV_INLINE Stream(const short* p, int64_t stride, int D)
-      : base(p), ss(stride) {
-    const int slot = threadIdx.x % L::kSlots;
-    col = slot * 8 < D ? slot * 16 : 0;
-    off = (threadIdx.x / L::kSlots) * static_cast<unsigned>(2 * stride) + col;
-  }
-  // rows past S: the last one, which `store` leaves out
-  DEV_INLINE void load(int t0, int S, s16x8 (&r)[L::kPer]) const {
+  DEV_INLINE Stream(const short* p, int64_t stride) : base(p), ss(stride) {}
+
+  // A tile of which every row is there and none is padding, and D == DP:
+  // straight from memory into LDS.  A wave's 16 bytes a lane land side by
+  // side, so the permutation of slots is in what a lane fetches.  No registers
+  // hold the tile on its way; the barrier before it is read waits for it.
+  DEV_INLINE void send(char* lds, int t0) const {
+    const int row = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
+    const unsigned step = static_cast<unsigned>(2 * ss);
+    // the permutation goes by the row's lowest three bits, which all passes
+    // share: kStep is a multiple of 8
+    const unsigned off =
+        row * step + ((L::at(row, slot) - row * (DP * 2)));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const char* p = reinterpret_cast<const char*>(base + t0 * ss);
-    const unsigned row = static_cast<unsigned>(2 * ss);
-    unsigned at[L::kPer];
-#pragma unroll
-    for (int i = 0; i < L::kPer; ++i) at[i] = off + i * L::kStep * row;
-    if (t0 + kTile > S) {
-#pragma unroll
-      for (int i = 0; i < L::kPer; ++i)
-        at[i] = static_cast<unsigned>(min(
-                    static_cast<int>(threadIdx.x) / L::kSlots + i * L::kStep,
-                    S - 1 - t0)) * row + col;
-    }
 #pragma unroll
     for (int i = 0; i < L::kPer; ++i)
-      r[i] = *reinterpret_cast<const s16x8*>(p + at[i]);
+      __builtin_amdgcn_global_load_lds(
+          (global_void*)(p + off + i * L::kStep * step),
+          (lds_void*)(lds + i * 4096 + wave * 1024), 16, 0, 0);
   }
-  // Into LDS.  some: rows that `live` has no bit of, and columns past D, become
-  // zeros.
-  DEV_INLINE static void store(char* lds, bool some, unsigned long long live,
-                               int D, const s16x8 (&r)[L::kPer]) {
-    const int row = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
-    if (some) {
+  // Any tile: rows that `live` has no bit of, and columns past D, as zeros.
+  DEV_INLINE void copy(char* lds, int t0, int S, int D,
+                       unsigned long long live) const {
+    const int row0 = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
+    const unsigned step = static_cast<unsigned>(2 * ss);
+    const char* p = reinterpret_cast<const char*>(base + t0 * ss);
 #pragma unroll
-      for (int i = 0; i < L::kPer; ++i) {
-        const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-        const bool keep =
-            slot * 8 < D && ((live >> (row + i * L::kStep)) & 1);
-        *reinterpret_cast<s16x8*>(lds + L::at(row + i * L::kStep, slot)) =
-            keep ? r[i] : zero;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < L::kPer; ++i)
-        *reinterpret_cast<s16x8*>(lds + L::at(row + i * L::kStep, slot)) =
-            r[i];
+    for (int i = 0; i < L::kPer; ++i) {
+      const int row = row0 + i * L::kStep;
+      s16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (slot * 8 < D && ((live >> row) & 1))
+        x = *reinterpret_cast<const s16x8*>(p + row * step + slot * 16);
+      *reinterpret_cast<s16x8*>(lds + L::at(row, slot)) = x;
     }
   }
 };
@@ -314,9 +305,10 @@ DEV_INLINE const int4* summary_of(const MaskedAttn& a, int n, int4* lds) {
 }
 
 // Lists the tiles of [base, base + kList) that meet the owned tokens from own0
-// on, in order: tile << 16, and two bits (`meet`) for every 32 owned tokens g
-// and either half of the tile: bits 4 g + 2 half.  Called by the whole
-// workgroup.
+// on, in order: (tile - base) << 17; kZeros if rows of the tile have to be
+// staged as zeros (padding, or none there); and two bits (`meet`) for every
+// 32 owned tokens g and either half of the tile: bits 4 g + 2 half.  Called by
+// the whole workgroup.
 template <bool OWN_Q, int GROUPS>
 DEV_INLINE int list_tiles(const MaskedAttn& a, int n, int own0, int base,
                           const int4* sum, unsigned* list, int* count) {
@@ -336,11 +328,13 @@ DEV_INLINE int list_tiles(const MaskedAttn& a, int n, int own0, int base,
     for (int t0 = base; t0 < end; t0 += kWave) {
       const int t = t0 + lane;
       unsigned c = 0;
+      int pad = 0;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int4 other =
             docs ? sum[min(t * 2 + hf, last)] : make_int4(0, 0, 0, 0);
         const int s0 = t * kTile + hf * 32;
+        pad |= other.z;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
           const int o0 = own0 + g * 32;
@@ -356,7 +350,8 @@ DEV_INLINE int list_tiles(const MaskedAttn& a, int n, int own0, int base,
       const unsigned long long hit = __ballot(c != 0);
       if (c != 0)
         list[found + __popcll(hit & ((1ull << lane) - 1))] =
-            (static_cast<unsigned>(t) << 16) | c;
+            (static_cast<unsigned>(t - base) << 17) | c |
+            (pad != 0 || (t + 1) * kTile > a.S ? kZeros : 0);
       found += __popcll(hit);
     }
     if (lane == 0) *count = found;
@@ -368,10 +363,8 @@ DEV_INLINE int list_tiles(const MaskedAttn& a, int n, int own0, int base,
 DEV_INLINE unsigned entry_of(const unsigned* list, int e, int count) {
   return __builtin_amdgcn_readfirstlane(list[min(e, count - 1)]);
 }
-DEV_INLINE int first_of(unsigned entry) { return (entry >> 16) * kTile; }
-// whether rows of a tile may have to be staged as zeros
-DEV_INLINE bool ragged(unsigned entry, int S) {
-  return (entry & 0x5555u) != 0 || first_of(entry) + kTile > S;
+DEV_INLINE int first_of(unsigned entry, int base) {
+  return (base + static_cast<int>(entry >> 17)) * kTile;
 }
 
 // document of an owned token: -1 for padding and past the end, 0 without

@@ -28,8 +28,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
   const int lim = pair_limit<true>(a, n, own);
   Docs docs(a, n);
   const int4* sum = summary_of(a, n, sm.sum);
-  const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss, a.D);
-  const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss, a.D);
+  const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss);
+  const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss);
   s16x8 qf[DP / 16], gf[DP / 16];
   own_rows<DP>(row_of(a.q, n, h) + own * a.q.ss, live, a.D, qf);
   own_rows<DP>(row_of(a.go, n, h) + own * a.go.ss, live, a.D, gf);
@@ -63,31 +63,34 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
     const int count = list_tiles<true, OWN / 32>(a, n, own0, base, sum,
                                                  sm.list, &sm.count);
     if (count == 0) continue;
-    s16x8 kr[L::kPer], vr[L::kPer];
-    auto fetch = [&](unsigned entry) {
-      const int t0 = first_of(entry);
-      ks.load(t0, a.S, kr);
-      vs.load(t0, a.S, vr);
+    // what of a tile goes ahead, and what is left for when its turn is near
+    auto fetch = [&](int buf, unsigned entry) {
+      const int t0 = first_of(entry, base);
       docs.load(t0, a.S);
+      if (!(entry & kZeros) && a.D == DP) {
+        ks.send(sm.tile[buf][0], t0);
+        vs.send(sm.tile[buf][1], t0);
+      }
     };
     auto keep = [&](int buf, unsigned entry) {
-      const int t0 = first_of(entry);
-      const bool some = ragged(entry, a.S) || a.D < DP;
-      const unsigned long long live = docs.live(t0, a.S);
-      Stream<DP>::store(sm.tile[buf][0], some, live, a.D, kr);
-      Stream<DP>::store(sm.tile[buf][1], some, live, a.D, vr);
+      const int t0 = first_of(entry, base);
+      if ((entry & kZeros) || a.D != DP) {
+        const unsigned long long live = docs.live(t0, a.S);
+        ks.copy(sm.tile[buf][0], t0, a.S, a.D, live);
+        vs.copy(sm.tile[buf][1], t0, a.S, a.D, live);
+      }
       if (threadIdx.x < kTile) sm.doc[buf][threadIdx.x] = docs.own(t0, a.S);
     };
     unsigned entry = entry_of(sm.list, 0, count);
     unsigned next = entry_of(sm.list, 1, count);
-    fetch(entry);
+    fetch(0, entry);
     keep(0, entry);
     __syncthreads();
     for (int e = 0; e < count; ++e) {
       const int buf = e & 1;
-      if (e + 1 < count) fetch(next);
+      if (e + 1 < count) fetch(buf ^ 1, next);
       const unsigned after = sm.list[min(e + 2, count - 1)];
-      const int t0 = first_of(entry);
+      const int t0 = first_of(entry, base);
       const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
 #pragma unroll
       for (int i = 0; i < KB; ++i) {
@@ -184,27 +187,29 @@ masked_attn_dkv_kernel(MaskedAttn a) {
     for (int hi = 0; hi < group && count > 0; ++hi) {
       const int h = hk * group + hi;
       const Score<M> sc(a, h);
-      const Stream<DP> qs(row_of(a.q, n, h), a.q.ss, a.D);
-      const Stream<DP> gs(row_of(a.go, n, h), a.go.ss, a.D);
+      const Stream<DP> qs(row_of(a.q, n, h), a.q.ss);
+      const Stream<DP> gs(row_of(a.go, n, h), a.go.ss);
       const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S;
-      s16x8 qr[L::kPer], gr[L::kPer];
       float lr, er;
-      auto fetch = [&](unsigned entry) {
-        const int t0 = first_of(entry);
-        qs.load(t0, a.S, qr);
-        gs.load(t0, a.S, gr);
+      auto fetch = [&](int buf, unsigned entry) {
+        const int t0 = first_of(entry, base);
         docs.load(t0, a.S);
+        if (!(entry & kZeros) && a.D == DP) {
+          qs.send(sm.tile[buf][0], t0);
+          gs.send(sm.tile[buf][1], t0);
+        }
         const int tok =
             min(t0 + static_cast<int>(threadIdx.x) % kTile, a.S - 1);
         lr = a.lse[stat + tok];
         er = a.delta[stat + tok];
       };
       auto keep = [&](int buf, unsigned entry) {
-        const int t0 = first_of(entry);
-        const bool some = ragged(entry, a.S) || a.D < DP;
-        const unsigned long long live = docs.live(t0, a.S);
-        Stream<DP>::store(sm.tile[buf][0], some, live, a.D, qr);
-        Stream<DP>::store(sm.tile[buf][1], some, live, a.D, gr);
+        const int t0 = first_of(entry, base);
+        if ((entry & kZeros) || a.D != DP) {
+          const unsigned long long live = docs.live(t0, a.S);
+          qs.copy(sm.tile[buf][0], t0, a.S, a.D, live);
+          gs.copy(sm.tile[buf][1], t0, a.S, a.D, live);
+        }
         if (threadIdx.x < kTile) {
           const bool past = t0 + static_cast<int>(threadIdx.x) >= a.S;
           sm.doc[buf][threadIdx.x] = docs.own(t0, a.S);
@@ -214,14 +219,14 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       };
       unsigned entry = entry_of(sm.list, 0, count);
       unsigned next = entry_of(sm.list, 1, count);
-      fetch(entry);
+      fetch(0, entry);
       keep(0, entry);
       __syncthreads();
       for (int e = 0; e < count; ++e) {
         const int buf = e & 1;
-        if (e + 1 < count) fetch(next);
+        if (e + 1 < count) fetch(buf ^ 1, next);
         const unsigned after = sm.list[min(e + 2, count - 1)];
-        const int t0 = first_of(entry);
+        const int t0 = first_of(entry, base);
         const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
 #pragma unroll
         for (int i = 0; i < KB; ++i) {

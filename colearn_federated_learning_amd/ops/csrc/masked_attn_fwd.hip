@@ -41,8 +41,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
   const int lim = pair_limit<true>(a, n, own);
   Docs docs(a, n);
   const int4* sum = summary_of(a, n, sm.sum);
-  const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss, a.D);
-  const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss, a.D);
+  const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss);
+  const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss);
   s16x8 qf[DP / 16];
   own_rows<DP>(row_of(a.q, n, h) + own * a.q.ss, live, a.D, qf);
   const Score<M> sc(a, h);
@@ -96,31 +96,34 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
     const int count = list_tiles<true, OWN / 32>(a, n, own0, base, sum,
                                                  sm.list, &sm.count);
     if (count == 0) continue;
-    s16x8 kr[L::kPer], vr[L::kPer];
-    auto fetch = [&](unsigned entry) {
-      const int t0 = first_of(entry);
-      ks.load(t0, a.S, kr);
-      vs.load(t0, a.S, vr);
+    // what of a tile goes ahead, and what is left for when its turn is near
+    auto fetch = [&](int buf, unsigned entry) {
+      const int t0 = first_of(entry, base);
       docs.load(t0, a.S);
+      if (!(entry & kZeros) && a.D == DP) {
+        ks.send(sm.tile[buf][0], t0);
+        vs.send(sm.tile[buf][1], t0);
+      }
     };
     auto keep = [&](int buf, unsigned entry) {
-      const int t0 = first_of(entry);
-      const bool some = ragged(entry, a.S) || a.D < DP;
-      const unsigned long long live = docs.live(t0, a.S);
-      Stream<DP>::store(sm.tile[buf][0], some, live, a.D, kr);
-      Stream<DP>::store(sm.tile[buf][1], some, live, a.D, vr);
+      const int t0 = first_of(entry, base);
+      if ((entry & kZeros) || a.D != DP) {
+        const unsigned long long live = docs.live(t0, a.S);
+        ks.copy(sm.tile[buf][0], t0, a.S, a.D, live);
+        vs.copy(sm.tile[buf][1], t0, a.S, a.D, live);
+      }
       if (threadIdx.x < kTile) sm.doc[buf][threadIdx.x] = docs.own(t0, a.S);
     };
     unsigned entry = entry_of(sm.list, 0, count);
     unsigned next = entry_of(sm.list, 1, count);
-    fetch(entry);
+    fetch(0, entry);
     keep(0, entry);
     __syncthreads();
     for (int e = 0; e < count; ++e) {
       const int buf = e & 1;
-      if (e + 1 < count) fetch(next);
+      if (e + 1 < count) fetch(buf ^ 1, next);
       const unsigned after = sm.list[min(e + 2, count - 1)];
-      const int t0 = first_of(entry);
+      const int t0 = first_of(entry, base);
       const char* kt = sm.tile[buf][0];
       const char* vt = sm.tile[buf][1];
       const int* dt = sm.doc[buf];
