@@ -462,6 +462,13 @@ void masked_attn_bwd(torch::Tensor go, torch::Tensor q, torch::Tensor k,
   a.lse = lse.data_ptr<float>();
   a.delta = delta.data_ptr<float>();
   if (sum.numel() > 0) a.tiles = reinterpret_cast<int4*>(sum.data_ptr<int>());
+  a.shares = masked_attn_shares(a);
+  torch::Tensor partial;
+  if (a.shares > 1) {
+    partial = torch::empty({2, a.shares, a.N, a.S, a.Hkv, a.D},
+                           lse.options());
+    a.partial = partial.data_ptr<float>();
+  }
   launch_masked_attn_bwd(a, elem_of(q, "q"), stream());
   HIP_CHECK_LAST();
 }

@@ -100,13 +100,21 @@ struct MaskedAttn {
   int4* tiles;                // [N, ceil(S / 32)] summary of doc, or null
   float* lse;                 // [N, H, S], base 2; +inf for empty rows
   float* delta;               // [N, H, S], backward only
+  float* partial;             // [2, shares, N, S, Hkv, D], if shares > 1
+  int shares;                 // of a key head's heads, backward only
   int N, S, H, Hkv, D;
   bool causal;
   float scale, softcap;
 };
 
-// whether two waves share 32 owned tokens, for a grid of `heads` a sequence
-bool masked_attn_split(const MaskedAttn& a, int heads);
+// Whether two waves share 32 owned tokens: if `heads` a sequence and 128 tokens
+// a workgroup make fewer than per_cu workgroups a CU.  Both sides measured,
+// 12 heads of size 64, us with two waves / with one: forward 1 x 4096 tokens
+// (384 workgroups) 79 / 94, 2 x 4096 (768) 161 / 136; dq 98 / 117 and
+// 198 / 172; dk/dv 1 x 2048 (192) 46 / 56, 1 x 4096 (384) 155 / 141.
+bool masked_attn_split(const MaskedAttn& a, int heads, int per_cu);
+// into how many shares dk/dv divides the heads of a key head
+int masked_attn_shares(const MaskedAttn& a);
 void launch_masked_attn_tiles(const MaskedAttn& a, hipStream_t stream);
 void launch_masked_attn_fwd(const MaskedAttn& a, Elem type,
                             hipStream_t stream);

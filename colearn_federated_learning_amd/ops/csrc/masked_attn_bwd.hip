@@ -159,9 +159,11 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   using L = Tile<DP>;
   constexpr int OWN = 128 / KS, KB = 2 / KS;
   __shared__ __align__(16) Smem<DP> sm;
-  int n, hk, own0;
-  locate<OWN>(a, a.Hkv, false, &n, &hk, &own0);
-  const int group = a.H / a.Hkv;
+  int n, hs, own0;  // hs: key head and share
+  locate<OWN>(a, a.Hkv * a.shares, false, &n, &hs, &own0);
+  const int hk = hs / a.shares, share = hs % a.shares;
+  // the heads of the group that this workgroup adds up: all, or its share
+  const int group = a.H / a.Hkv / a.shares;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
@@ -179,13 +181,67 @@ masked_attn_dkv_kernel(MaskedAttn a) {
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = 0.f;
 
+  // half qb of the streamed tile; mixed: some pairs of it are not attended
+  auto work = [&](const Score<M>& sc, int buf, int qb, int t0, bool mixed) {
+    const char* qt = sm.tile[buf][0] + qb * (L::kBytes / 2);
+    const char* gt = sm.tile[buf][1] + qb * (L::kBytes / 2);
+    const int other = qb * 32 + 4 * half;
+    f32x16 z = 0.f, dp = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      z = mfma<T>(L::rows(qt, kk), kf[kk], z);
+      dp = mfma<T>(L::rows(gt, kk), vf[kk], dp);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 de =
+          *reinterpret_cast<const float4*>(sm.delta[buf] + other + g * 8);
+      dp[g * 4] -= de.x;
+      dp[g * 4 + 1] -= de.y;
+      dp[g * 4 + 2] -= de.z;
+      dp[g * 4 + 3] -= de.w;
+    }
+    if constexpr (M == kCap) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float th = fast_tanh(z[r] * sc.cap_in);
+        dp[r] *= 1.f - th * th;
+      }
+    }
+    sc.shape(z, static_cast<float>(own - t0 - other));
+    if (mixed)
+      mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 ls =
+          *reinterpret_cast<const float4*>(sm.lse[buf] + other + g * 8);
+      const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = g * 4 + j;
+        z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -l4[j]));
+        dp[r] *= z[r];
+        z[r] *= kLift<T>;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const s16x8 p = round8<T>(z, s);
+      const s16x8 x = round8<T>(dp, s);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        dv[db] = mfma<T>(L::cols(gt, s, db), p, dv[db]);
+        dk[db] = mfma<T>(L::cols(qt, s, db), x, dk[db]);
+      }
+    }
+  };
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
     const int count = list_tiles<false, OWN / 32>(a, n, own0, base, sum,
                                                   sm.list, &sm.count);
     // every head of the group over the same list, one after another
     for (int hi = 0; hi < group && count > 0; ++hi) {
-      const int h = hk * group + hi;
+      const int h = hs * group + hi;
       const Score<M> sc(a, h);
       const Stream<DP> qs(row_of(a.q, n, h), a.q.ss);
       const Stream<DP> gs(row_of(a.go, n, h), a.go.ss);
@@ -232,58 +288,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
         for (int i = 0; i < KB; ++i) {
           const int qb = KS == 1 ? i : part;
           const unsigned c = (cls >> (2 * qb)) & 3;
-          if (c == 0) continue;
-          const char* qt = sm.tile[buf][0] + qb * (L::kBytes / 2);
-          const char* gt = sm.tile[buf][1] + qb * (L::kBytes / 2);
-          const int other = qb * 32 + 4 * half;
-          f32x16 z = 0.f, dp = 0.f;
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            z = mfma<T>(L::rows(qt, kk), kf[kk], z);
-            dp = mfma<T>(L::rows(gt, kk), vf[kk], dp);
-          }
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float4 de = *reinterpret_cast<const float4*>(
-                sm.delta[buf] + other + g * 8);
-            dp[g * 4] -= de.x;
-            dp[g * 4 + 1] -= de.y;
-            dp[g * 4 + 2] -= de.z;
-            dp[g * 4 + 3] -= de.w;
-          }
-          if constexpr (M == kCap) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float th = fast_tanh(z[r] * sc.cap_in);
-              dp[r] *= 1.f - th * th;
-            }
-          }
-          sc.shape(z, static_cast<float>(own - t0 - other));
-          if (c == 1)
-            mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float4 ls = *reinterpret_cast<const float4*>(
-                sm.lse[buf] + other + g * 8);
-            const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int r = g * 4 + j;
-              z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -l4[j]));
-              dp[r] *= z[r];
-              z[r] *= kLift<T>;
-            }
-          }
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const s16x8 p = round8<T>(z, s);
-            const s16x8 x = round8<T>(dp, s);
-#pragma unroll
-            for (int db = 0; db < DP / 32; ++db) {
-              dv[db] = mfma<T>(L::cols(gt, s, db), p, dv[db]);
-              dk[db] = mfma<T>(L::cols(qt, s, db), x, dk[db]);
-            }
-          }
+          if (c != 0) work(sc, buf, qb, t0, c == 1);
         }
         if (e + 1 < count) keep(buf ^ 1, next);
         entry = next;
@@ -310,7 +315,14 @@ masked_attn_dkv_kernel(MaskedAttn a) {
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dv[i] += o[i];
   }
-  if (own < a.S) {
+  if (own < a.S && a.shares > 1) {
+    const int64_t size = static_cast<int64_t>(a.N) * a.S * a.Hkv * a.D;
+    float* at = a.partial + share * size +
+                ((static_cast<int64_t>(n) * a.S + own) * a.Hkv + hk) * a.D;
+    store_cols<float, DP>(at, dk, a.scale, live, a.D);
+    store_cols<float, DP>(at + a.shares * size, dv, 1.f / kLift<T>, live,
+                          a.D);
+  } else if (own < a.S) {
     store_cols<T, DP>(static_cast<T*>(a.gk.p) + n * a.gk.sn + own * a.gk.ss +
                           hk * a.gk.sh,
                       dk, a.scale, live, a.D);
@@ -320,28 +332,74 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   }
 }
 
+// Shares' sums, four elements a thread: grid.y 0 dk, 1 dv.
+template <typename T>
+__global__ __launch_bounds__(256) void masked_attn_join_kernel(MaskedAttn a) {
+  const int64_t size = static_cast<int64_t>(a.N) * a.S * a.Hkv * a.D;
+  const int64_t i =
+      (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= size) return;
+  const float* p = a.partial + blockIdx.y * a.shares * size + i;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < a.shares; ++k) {
+    float y[4];
+    elem_load4(p + k * size, y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] += y[j];
+  }
+  const HeadView& v = blockIdx.y == 0 ? a.gk : a.gv;
+  const int64_t row = i / a.D;  // (n S + token) Hkv + head
+  const int col = static_cast<int>(i - row * a.D);
+  const int64_t tok = row / a.Hkv;
+  const int h = static_cast<int>(row - tok * a.Hkv);
+  const int64_t n = tok / a.S;
+  elem_store4(static_cast<T*>(v.p) + n * v.sn + (tok - n * a.S) * v.ss +
+                  h * v.sh + col,
+              x);
+}
+
 struct Backward {
   const MaskedAttn& a;
   hipStream_t stream;
 
   template <typename T, int DP, Mode M>
   void run() const {
-    if (masked_attn_split(a, a.H))
+    if (masked_attn_split(a, a.H, 2))
       masked_attn_dq_kernel<T, DP, M, 2>
           <<<a.N * a.H * ((a.S + 63) / 64), 256, 0, stream>>>(a);
     else
       masked_attn_dq_kernel<T, DP, M, 1>
           <<<a.N * a.H * ((a.S + 127) / 128), 256, 0, stream>>>(a);
-    if (masked_attn_split(a, a.Hkv))
+    const int heads = a.Hkv * a.shares;
+    if (masked_attn_split(a, heads, 1))
       masked_attn_dkv_kernel<T, DP, M, 2>
-          <<<a.N * a.Hkv * ((a.S + 63) / 64), 256, 0, stream>>>(a);
+          <<<a.N * heads * ((a.S + 63) / 64), 256, 0, stream>>>(a);
     else
       masked_attn_dkv_kernel<T, DP, M, 1>
-          <<<a.N * a.Hkv * ((a.S + 127) / 128), 256, 0, stream>>>(a);
+          <<<a.N * heads * ((a.S + 127) / 128), 256, 0, stream>>>(a);
+    if (a.shares > 1) {
+      const int64_t size = static_cast<int64_t>(a.N) * a.S * a.Hkv * a.D;
+      masked_attn_join_kernel<T>
+          <<<dim3(static_cast<unsigned>((size / 4 + 255) / 256), 2), 256, 0,
+             stream>>>(a);
+    }
   }
 };
 
 }  // namespace
+
+int masked_attn_shares(const MaskedAttn& a) {
+  // Key heads that serve several heads leave the dk/dv grid short: the group
+  // is shared out until there are two workgroups a CU, or every head has its
+  // own.  2 x 1999 capped tokens, 16 heads over 4, size 128:
+  // 281 us in one share, 227 + 13 (the join) in four.
+  const int group = a.H / a.Hkv;
+  const int64_t blocks =
+      static_cast<int64_t>(a.N) * a.Hkv * ((a.S + 127) / 128);
+  for (int k = 1; k < group; ++k)
+    if (group % k == 0 && blocks * k >= 2 * kNumCU) return k;
+  return group;
+}
 
 void launch_masked_attn_bwd(const MaskedAttn& a, Elem type,
                             hipStream_t stream) {

@@ -185,7 +185,7 @@ struct Forward {
   template <typename T, int DP, Mode M>
   void run() const {
     const int heads = a.N * a.H;
-    if (masked_attn_split(a, a.H))
+    if (masked_attn_split(a, a.H, 2))
       masked_attn_fwd_kernel<T, DP, M, 2>
           <<<heads * ((a.S + 63) / 64), 256, 0, stream>>>(a);
     else
@@ -196,10 +196,10 @@ struct Forward {
 
 }  // namespace
 
-bool masked_attn_split(const MaskedAttn& a, int heads) {
+bool masked_attn_split(const MaskedAttn& a, int heads, int per_cu) {
   const int64_t blocks =
       static_cast<int64_t>(a.N) * heads * ((a.S + 127) / 128);
-  return blocks < 2 * kNumCU;
+  return blocks < per_cu * kNumCU;
 }
 
 void launch_masked_attn_tiles(const MaskedAttn& a, hipStream_t stream) {
