@@ -100,49 +100,6 @@ def _masked_attention_ref(q, k, v, scale, causal, softcap, prefix, doc,
     return out.transpose(1, 2).to(q.dtype)
 
 
-class _MaskedAttnFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, args, prefix, doc, slopes):
-        out, lse, tiles = require_ext().masked_attn_fwd(
-            q, k, v, *args, prefix, doc, slopes)
-        ctx.save_for_backward(q, k, v, out, lse, tiles, prefix, doc, slopes)
-        ctx.args = args
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, go):
-        q, k, v, out, lse, tiles, prefix, doc, slopes = ctx.saved_tensors
-        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                      for t in (q, k, v))
-        require_ext().masked_attn_bwd(go, q, k, v, out, lse, tiles, gq, gk,
-                                      gv, *ctx.args, prefix, doc, slopes)
-        return gq, gk, gv, None, None, None, None
-
-
-class _MaskedAttnQKVFn(torch.autograd.Function):
-    """The fused projection's layout: one gradient tensor, written in place
-    of three that autograd would have to put together."""
-
-    @staticmethod
-    def forward(ctx, qkv, args, prefix, doc, slopes):
-        out, lse, tiles = require_ext().masked_attn_fwd(
-            *qkv.unbind(2), *args, prefix, doc, slopes)
-        ctx.save_for_backward(qkv, out, lse, tiles, prefix, doc, slopes)
-        ctx.args = args
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, go):
-        qkv, out, lse, tiles, prefix, doc, slopes = ctx.saved_tensors
-        g = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        require_ext().masked_attn_bwd(go, *qkv.unbind(2), out, lse, tiles,
-                                      *g.unbind(2), *ctx.args, prefix, doc,
-                                      slopes)
-        return g, None, None, None, None
-
-
 def _check_masked(q, k, v, scale, causal, softcap, prefix, doc, slopes):
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or (
             q.shape[0] != k.shape[0] or q.shape[1] != k.shape[1]
@@ -227,9 +184,8 @@ def colearn_attention(
     if not _masked_native(q, k, v):
         return _masked_attention_ref(q, k, v, scale, causal, softcap, prefix,
                                      doc, slopes)
-    return _MaskedAttnFn.apply(
-        q, k, v, (float(scale), bool(causal), float(softcap)),
-        *_contiguous(prefix, doc, slopes))
+    return require_ext().masked_attention(q, k, v, scale, causal, softcap,
+                                          *_contiguous(prefix, doc, slopes))
 
 
 def colearn_attention_qkv(
@@ -253,9 +209,8 @@ def colearn_attention_qkv(
         out = _masked_attention_ref(q, k, v, scale, causal, softcap, prefix,
                                     doc, slopes)
     else:
-        out = _MaskedAttnQKVFn.apply(
-            qkv, (float(scale), bool(causal), float(softcap)),
-            *_contiguous(prefix, doc, slopes))
+        out = require_ext().masked_attention_qkv(
+            qkv, scale, causal, softcap, *_contiguous(prefix, doc, slopes))
     return out.flatten(2)
 
 

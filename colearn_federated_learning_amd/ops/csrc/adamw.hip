@@ -141,8 +141,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTable tab,
       }
     }
     if constexpr (EIGHT) {
-      top_m = wave_allreduce_max(top_m);
-      top_v = wave_allreduce_max(top_v);
+      top_m = lanes_max(top_m);
+      top_v = lanes_max(top_v);
       const float inv_m = top_m > kTiny ? kE4M3Max / top_m : 0.f;
       const float inv_v = top_v > kTiny ? kE4M3Max / top_v : 0.f;
       if (lane == 0) {

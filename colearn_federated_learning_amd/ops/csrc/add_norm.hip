@@ -28,7 +28,7 @@ namespace {
 template <int W, int N>
 DEV_INLINE void row_sum(float (&v)[N], float (*red)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_allreduce_sum(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i]);
   if constexpr (W > 1) {
     const int wave = threadIdx.x / kWave;
     if (threadIdx.x % kWave == 0) {
@@ -52,6 +52,25 @@ template <int VEC, int W>
 DEV_INLINE int col_of(int k) {
   const int wave = W > 1 ? threadIdx.x / kWave : 0;
   return ((k * W + wave) * kWave + threadIdx.x % kWave) * VEC;
+}
+
+// a vector as it lies in memory, and its values
+template <typename T, int VEC>
+struct Raw {
+  T x[VEC];
+};
+template <typename T>
+struct alignas(4 * sizeof(T)) Raw<T, 4> {
+  T x[4];
+};
+template <int VEC, typename T>
+DEV_INLINE Raw<T, VEC> load_raw(const T* p) {
+  return *reinterpret_cast<const Raw<T, VEC>*>(p);
+}
+template <int VEC, typename T>
+DEV_INLINE void widen(const Raw<T, VEC>& r, float* x) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) x[j] = elem_load(&r.x[j]);
 }
 
 template <int VEC, typename T>
@@ -158,25 +177,44 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void add_norm_bwd_kernel(
     if (c < H) load_vec<VEC>(w + c, wv + k * VEC);
   }
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * rpg;
-  for (int64_t q = static_cast<int64_t>(blockIdx.x) * kRows +
-                   (W == 1 ? threadIdx.x / kWave : 0);
-       q < rpg; q += static_cast<int64_t>(gridDim.x) * kRows) {
-    const int64_t row = row0 + q;
-    const float mu = mean[row], is = inv[row];
-    float g[EL], xh[EL];
-    float sum[2] = {0.f, 0.f};
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t q = static_cast<int64_t>(blockIdx.x) * kRows +
+              (W == 1 ? threadIdx.x / kWave : 0);
+  // The next row's loads are under way while a row is reduced and written
+  // (not where 16 waves leave no registers for them).
+  constexpr bool kAhead = W < 16;
+  Raw<T, VEC> gr[NV], sr[NV];
+  float mu = 0.f, is = 0.f;
+  auto fetch = [&](int64_t row) {
+    mu = mean[row];
+    is = inv[row];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = col_of<VEC, W>(k);
+      const int c = min(col_of<VEC, W>(k), H - VEC);
+      gr[k] = load_raw<VEC>(gy + row * H + c);
+      sr[k] = load_raw<VEC>(s + row * H + c);
+    }
+  };
+  if (kAhead && q < rpg) fetch(row0 + q);
+  for (; q < rpg; q += stride) {
+    const int64_t row = row0 + q;
+    if (!kAhead) fetch(row);
+    float g[EL], xh[EL];
+    float sum[2] = {0.f, 0.f};
+    const float m = mu, rs = is;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) g[k * VEC + j] = xh[k * VEC + j] = 0.f;
-      if (c < H) {
-        load_vec<VEC>(gy + row * H + c, g + k * VEC);
-        load_vec<VEC>(s + row * H + c, xh + k * VEC);
+    for (int k = 0; k < NV; ++k) {
+      widen<VEC>(gr[k], g + k * VEC);
+      widen<VEC>(sr[k], xh + k * VEC);
+    }
+    if (kAhead && q + stride < rpg) fetch(row + stride);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (col_of<VEC, W>(k) < H) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int e = k * VEC + j;
-          xh[e] = (xh[e] - mu) * is;
+          xh[e] = (xh[e] - m) * rs;
           ab[e] += g[e];
           aw[e] += g[e] * xh[e];
           g[e] *= wv[e];
@@ -196,7 +234,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void add_norm_bwd_kernel(
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int e = k * VEC + j;
-          o[j] = is * (g[e] - sum[0] - xh[e] * sum[1]);
+          o[j] = rs * (g[e] - sum[0] - xh[e] * sum[1]);
         }
         if (gs != nullptr) {
           float u[VEC];
@@ -341,11 +379,14 @@ void pick(const NormArgs& a, Elem type, bool vec, int H) {
 }  // namespace
 
 int add_norm_parts(int64_t rows, int groups, int H) {
-  // A workgroup should carry rows enough to pay for its row of partial sums:
-  // at least 4 a wave, and 4 workgroups a CU over all groups.
+  // A row of partial sums costs as much as two thirds of a 16-bit data row:
+  // at least two rows a wave, and two workgroups a CU over all groups.  Rows
+  // of 768 in bf16, us with the join at 1 / 2 / 4 / 8 rows a wave: 4096 rows
+  // 14.2 / 11.7 / 12.6 / 15.5; 65536 rows at 2 / 4 / 8 workgroups a CU: 66 /
+  // 68 / 69.
   const int64_t rpg = rows / groups;
-  const int64_t per = H <= 16 * kWave ? 16 : 4;
-  const int64_t most = (4 * kNumCU + groups - 1) / groups;
+  const int64_t per = H <= 16 * kWave ? 8 : 2;
+  const int64_t most = (2 * kNumCU + groups - 1) / groups;
   int64_t n = (rpg + per - 1) / per;
   n = n < most ? n : most;
   return static_cast<int>(n > 0 ? n : 1);

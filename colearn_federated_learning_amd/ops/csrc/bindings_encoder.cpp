@@ -4,6 +4,8 @@
 
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <algorithm>
 #include <limits>
 #include <optional>
@@ -473,14 +475,187 @@ void masked_attn_bwd(torch::Tensor go, torch::Tensor q, torch::Tensor k,
   HIP_CHECK_LAST();
 }
 
+// ---- autograd -------------------------------------------------------------------
+// In C++: the engine's thread then needs no interpreter, which is most of a
+// small backward pass (norm of 4096 x 768, forward and backward: 115 us of
+// host time with functions in Python, BACKWARD here).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The kernels' gradients have no gradient of their own: asked for one
+// (create_graph), they raise when it is used, as once_differentiable's do.
+variable_list once(const char* name, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list there;
+  for (auto& g : grads)
+    if (g.defined()) there.push_back(g.detach().set_requires_grad(true));
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("trying to differentiate twice ") + name +
+          ", whose backward pass is a kernel",
+      static_cast<int64_t>(there.size()));
+  auto marked = (*error)(std::move(there));
+  size_t k = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = marked[k++];
+  return grads;
+}
+
+struct AddNormFn : public torch::autograd::Function<AddNormFn> {
+  static variable_list forward(AutogradContext* ctx, torch::Tensor x,
+                               OptTensor residual, torch::Tensor weight,
+                               torch::Tensor bias, double eps, int64_t groups,
+                               OptTensor gslot_w, OptTensor gslot_b) {
+    auto [y, s, mean, inv] =
+        add_norm_fwd(x, residual, weight, bias, eps, groups);
+    ctx->save_for_backward({s, weight, mean, inv,
+                            gslot_w.value_or(torch::Tensor()),
+                            gslot_b.value_or(torch::Tensor())});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["bias"] = bias.sizes().vec();
+    ctx->set_materialize_grads(false);
+    if (!residual.has_value()) s = s.view_as(s);  // no output is an input
+    return {y, s};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool residual = ctx->saved_data["residual"].toBool();
+    variable_list out(8);
+    torch::Tensor gx;
+    if (!grads[0].defined()) {  // only the sum was used
+      gx = grads[1];
+    } else {
+      const auto& weight = saved[1];
+      const bool direct = saved[4].defined();
+      auto gw = direct ? saved[4] : torch::empty_like(weight);
+      auto gb = direct ? saved[5]
+                       : torch::empty(ctx->saved_data["bias"].toIntVector(),
+                                      weight.options());
+      OptTensor gs;
+      if (grads[1].defined()) gs = grads[1].contiguous();
+      gx = add_norm_bwd(grads[0].contiguous(), gs, saved[0], weight, saved[2],
+                        saved[3], ctx->saved_data["groups"].toInt(), gw, gb);
+      if (!direct) {
+        out[2] = gw;
+        out[3] = gb;
+      }
+    }
+    out[0] = gx;
+    if (residual && ctx->needs_input_grad(1)) out[1] = gx;
+    return once("add + layer norm", std::move(out));
+  }
+};
+
+std::tuple<torch::Tensor, torch::Tensor> add_layer_norm(
+    torch::Tensor x, OptTensor residual, torch::Tensor weight,
+    torch::Tensor bias, double eps, int64_t groups, OptTensor gslot_w,
+    OptTensor gslot_b) {
+  auto out = AddNormFn::apply(x, residual, weight, bias, eps, groups, gslot_w,
+                              gslot_b);
+  return {out[0], out[1]};
+}
+
+void keep_masks(AutogradContext* ctx, double scale, bool causal,
+                double softcap, variable_list saved, const OptTensor& prefix,
+                const OptTensor& doc, const OptTensor& slopes) {
+  for (const auto& t : {prefix, doc, slopes})
+    saved.push_back(t.value_or(torch::Tensor()));
+  ctx->save_for_backward(std::move(saved));
+  ctx->saved_data["scale"] = scale;
+  ctx->saved_data["causal"] = causal;
+  ctx->saved_data["softcap"] = softcap;
+}
+
+void run_masked_bwd(AutogradContext* ctx, const torch::Tensor& go,
+                    const torch::Tensor& q, const torch::Tensor& k,
+                    const torch::Tensor& v, const variable_list& saved,
+                    size_t at, torch::Tensor gq, torch::Tensor gk,
+                    torch::Tensor gv) {
+  auto opt = [&](size_t i) -> OptTensor {
+    return saved[i].defined() ? OptTensor(saved[i]) : OptTensor();
+  };
+  masked_attn_bwd(go, q, k, v, saved[at], saved[at + 1], saved[at + 2], gq, gk,
+                  gv, ctx->saved_data["scale"].toDouble(),
+                  ctx->saved_data["causal"].toBool(),
+                  ctx->saved_data["softcap"].toDouble(), opt(at + 3),
+                  opt(at + 4), opt(at + 5));
+}
+
+struct MaskedAttnFn : public torch::autograd::Function<MaskedAttnFn> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor q,
+                               torch::Tensor k, torch::Tensor v, double scale,
+                               bool causal, double softcap, OptTensor prefix,
+                               OptTensor doc, OptTensor slopes) {
+    auto [o, lse, sum] = masked_attn_fwd(q, k, v, scale, causal, softcap,
+                                         prefix, doc, slopes);
+    keep_masks(ctx, scale, causal, softcap, {q, k, v, o, lse, sum}, prefix,
+               doc, slopes);
+    return o;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list out(9);
+    for (int i = 0; i < 3; ++i)
+      out[i] = torch::empty(saved[i].sizes(), saved[i].options());
+    run_masked_bwd(ctx, grads[0], saved[0], saved[1], saved[2], saved, 3,
+                   out[0], out[1], out[2]);
+    return once("masked attention", std::move(out));
+  }
+};
+
+// The fused projection's layout [N, S, 3, H, D]: one gradient tensor, written
+// in place of three that autograd would have to put together.
+struct MaskedAttnQKVFn : public torch::autograd::Function<MaskedAttnQKVFn> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor qkv,
+                               double scale, bool causal, double softcap,
+                               OptTensor prefix, OptTensor doc,
+                               OptTensor slopes) {
+    auto [o, lse, sum] =
+        masked_attn_fwd(qkv.select(2, 0), qkv.select(2, 1), qkv.select(2, 2),
+                        scale, causal, softcap, prefix, doc, slopes);
+    keep_masks(ctx, scale, causal, softcap, {qkv, o, lse, sum}, prefix, doc,
+               slopes);
+    return o;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto& qkv = saved[0];
+    variable_list out(7);
+    auto g = torch::empty(qkv.sizes(), qkv.options());
+    run_masked_bwd(ctx, grads[0], qkv.select(2, 0), qkv.select(2, 1),
+                   qkv.select(2, 2), saved, 1, g.select(2, 0), g.select(2, 1),
+                   g.select(2, 2));
+    out[0] = g;
+    return once("masked attention", std::move(out));
+  }
+};
+
+torch::Tensor masked_attention(torch::Tensor q, torch::Tensor k,
+                               torch::Tensor v, double scale, bool causal,
+                               double softcap, OptTensor prefix, OptTensor doc,
+                               OptTensor slopes) {
+  return MaskedAttnFn::apply(q, k, v, scale, causal, softcap, prefix, doc,
+                             slopes);
+}
+
+torch::Tensor masked_attention_qkv(torch::Tensor qkv, double scale,
+                                   bool causal, double softcap,
+                                   OptTensor prefix, OptTensor doc,
+                                   OptTensor slopes) {
+  return MaskedAttnQKVFn::apply(qkv, scale, causal, softcap, prefix, doc,
+                                slopes);
+}
+
 }  // namespace
 
 void bind_encoder(pybind11::module& m) {
   m.def("adamw_step", &adamw_step);
-  m.def("add_norm_fwd", &add_norm_fwd);
-  m.def("add_norm_bwd", &add_norm_bwd);
-  m.def("masked_attn_fwd", &masked_attn_fwd);
-  m.def("masked_attn_bwd", &masked_attn_bwd);
+  m.def("add_layer_norm", &add_layer_norm);
+  m.def("masked_attention", &masked_attention);
+  m.def("masked_attention_qkv", &masked_attention_qkv);
 }
 
 }  // namespace colearn

@@ -66,4 +66,44 @@ DEV_INLINE float elem_round(float x, const f16*) {
   return static_cast<float>(static_cast<f16>(x));
 }
 
+// ---- wave reductions in registers -------------------------------------------
+// Every lane gets the result; no LDS and no lane index arithmetic.  Exchanges
+// within 16 lanes are DPP moves (xor 1, xor 2, mirrored halves, mirrored row:
+// after each, the lanes that were joined agree), the last two swap rows.
+template <int CTRL>
+DEV_INLINE float dpp_move(float v) {
+  return __int_as_float(
+      __builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+DEV_INLINE float swap32(float v) {  // lane ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(
+      __float_as_int(v), __float_as_int(v), false, false);
+  return __int_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+DEV_INLINE float lanes_sum(float v) {
+  v += dpp_move<0xB1>(v);
+  v += dpp_move<0x4E>(v);
+  v += dpp_move<0x141>(v);
+  v += dpp_move<0x140>(v);
+  // a swap returns both sides: their sum is the same in either lane
+  const auto a = __builtin_amdgcn_permlane16_swap(
+      __float_as_int(v), __float_as_int(v), false, false);
+  v = __int_as_float(a[0]) + __int_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(
+      __float_as_int(v), __float_as_int(v), false, false);
+  return __int_as_float(b[0]) + __int_as_float(b[1]);
+}
+DEV_INLINE float lanes_max(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  v = fmaxf(v, dpp_move<0x140>(v));
+  const auto a = __builtin_amdgcn_permlane16_swap(
+      __float_as_int(v), __float_as_int(v), false, false);
+  v = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(
+      __float_as_int(v), __float_as_int(v), false, false);
+  return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+
 }  // namespace colearn

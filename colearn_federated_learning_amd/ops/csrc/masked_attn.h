@@ -113,7 +113,7 @@ DEV_INLINE float fast_tanh(float x) {
 }
 
 // the other half's value (lane ^ 32)
-DEV_INLINE float other_half(float x) { return __shfl_xor(x, 32); }
+DEV_INLINE float other_half(float x) { return swap32(x); }
 
 // A tile of kTile rows of DP 16-bit values.  16-byte slots are permuted
 // within a row so that neither read below hits a bank twice: eight

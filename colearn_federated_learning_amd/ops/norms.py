@@ -294,43 +294,6 @@ def _add_layer_norm_ref(x, residual, weight, bias, eps, groups):
     return y.to(x.dtype).reshape(x.shape), s
 
 
-class _AddLayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps, groups, gslot_w,
-                gslot_b):
-        y, s, mean, inv = require_ext().add_norm_fwd(
-            x, residual, weight, bias, eps, groups)
-        ctx.save_for_backward(s, weight, mean, inv)
-        ctx.groups = groups
-        ctx.gslots = (gslot_w, gslot_b)
-        ctx.bias_shape = bias.shape
-        ctx.set_materialize_grads(False)
-        if residual is None:
-            s = s.view_as(s)  # an input is not an output of its own
-        return y, s
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy, gs):
-        s, weight, mean, inv = ctx.saved_tensors
-        if gy is None:  # only the sum was used
-            return (gs, gs if ctx.needs_input_grad[1] else None, None, None,
-                    None, None, None, None)
-        gw, gb = ctx.gslots
-        direct = gw is not None
-        if not direct:
-            gw = torch.empty_like(weight)
-            gb = torch.empty(ctx.bias_shape, dtype=weight.dtype,
-                             device=weight.device)
-        gx = require_ext().add_norm_bwd(
-            gy.contiguous(), None if gs is None else gs.contiguous(), s,
-            weight, mean, inv, ctx.groups, gw, gb)
-        if direct:
-            gw = gb = None
-        return (gx, gx if ctx.needs_input_grad[1] else None, gw, gb, None,
-                None, None, None)
-
-
 def colearn_add_layer_norm(
     x: torch.Tensor, residual: Optional[torch.Tensor],
     weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-12,
@@ -383,7 +346,7 @@ def colearn_add_layer_norm(
         return _add_layer_norm_ref(x, residual, weight, bias, eps, groups)
     if weight.dtype != torch.float32 or bias.dtype != torch.float32:
         raise TypeError("weight and bias must be float32")
-    return _AddLayerNormFn.apply(
+    return require_ext().add_layer_norm(
         x.contiguous(),
         None if residual is None else residual.contiguous(),
         weight.contiguous(), bias.contiguous(), eps, groups, gslot_w,
