@@ -139,13 +139,10 @@ def _check_masked(q, k, v, scale, causal, softcap, prefix, doc, slopes):
 
 
 def _masked_native(q, *rest) -> bool:
-    return (q.is_cuda and native_enabled() and not is_vmapped(q, *rest)
-            and q.dtype in (torch.bfloat16, torch.float16)
-            and q.shape[-1] % 8 == 0 and 8 <= q.shape[-1] <= 128)
-
-
-def _contiguous(*ts):
-    return tuple(t if t is None else t.contiguous() for t in ts)
+    return (q.is_cuda and native_enabled()
+            and q.dtype in (torch.bfloat16, torch.float16) and q.dim() >= 4
+            and q.shape[-1] % 8 == 0 and 8 <= q.shape[-1] <= 128
+            and not is_vmapped(q, *rest))
 
 
 def colearn_attention(
@@ -180,12 +177,12 @@ def colearn_attention(
         q, k, v = q.to(dt), k.to(dt), v.to(dt)
     if scale is None:
         scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
+    if _masked_native(q, k, v):  # checks its operands itself
+        return require_ext().masked_attention(q, k, v, scale, causal, softcap,
+                                              prefix, doc, slopes)
     _check_masked(q, k, v, scale, causal, softcap, prefix, doc, slopes)
-    if not _masked_native(q, k, v):
-        return _masked_attention_ref(q, k, v, scale, causal, softcap, prefix,
-                                     doc, slopes)
-    return require_ext().masked_attention(q, k, v, scale, causal, softcap,
-                                          *_contiguous(prefix, doc, slopes))
+    return _masked_attention_ref(q, k, v, scale, causal, softcap, prefix, doc,
+                                 slopes)
 
 
 def colearn_attention_qkv(
@@ -203,15 +200,13 @@ def colearn_attention_qkv(
         qkv = qkv.to(torch.get_autocast_dtype("cuda"))
     if scale is None:
         scale = qkv.shape[-1] ** -0.5 if qkv.shape[-1] else 1.0
+    if _masked_native(qkv):  # checks its operands itself
+        return require_ext().masked_attention_qkv(qkv, scale, causal, softcap,
+                                                  prefix, doc, slopes)
     q, k, v = qkv.unbind(2)
     _check_masked(q, k, v, scale, causal, softcap, prefix, doc, slopes)
-    if not _masked_native(q, qkv):
-        out = _masked_attention_ref(q, k, v, scale, causal, softcap, prefix,
-                                    doc, slopes)
-    else:
-        out = require_ext().masked_attention_qkv(
-            qkv, scale, causal, softcap, *_contiguous(prefix, doc, slopes))
-    return out.flatten(2)
+    return _masked_attention_ref(q, k, v, scale, causal, softcap, prefix, doc,
+                                 slopes).flatten(2)
 
 
 def distance_slopes(heads: int, device=None) -> torch.Tensor:

@@ -318,31 +318,41 @@ MaskedAttn describe(const torch::Tensor& q, const torch::Tensor& k,
                     const torch::Tensor& v, double scale, bool causal,
                     double softcap, const OptTensor& prefix,
                     const OptTensor& doc, const OptTensor& slopes) {
-  TORCH_CHECK(q.is_cuda() && (q.scalar_type() == torch::kBFloat16 ||
-                              q.scalar_type() == torch::kFloat16),
-              "masked_attn: q must be a bfloat16 or float16 GPU tensor");
+  TORCH_CHECK_TYPE(q.is_cuda() && (q.scalar_type() == torch::kBFloat16 ||
+                                   q.scalar_type() == torch::kFloat16),
+                   "attention: q must be a bfloat16 or float16 GPU tensor");
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() &&
+                        q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+                        q.size(3) == k.size(3),
+                    "attention takes q [N, S, H, D] and k, v [N, S, Hkv, D], "
+                    "got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+  auto here = [&](const torch::Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.device() == q.device(), "attention: ", name, " on ",
+                      t.device(), ", q on ", q.device());
+  };
   for (const auto& t : {k, v}) {
-    check_gpu(t, q.device(), "masked_attn: k and v");
-    TORCH_CHECK(t.scalar_type() == q.scalar_type(),
-                "masked_attn: q, k and v must have one type");
+    TORCH_CHECK_TYPE(t.scalar_type() == q.scalar_type(),
+                     "attention: q, k and v must have one type, got ",
+                     q.scalar_type(), ", ", k.scalar_type(), ", ",
+                     v.scalar_type());
+    here(t, "k or v");
   }
-  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() &&
-                  q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
-                  q.size(3) == k.size(3),
-              "masked_attn: q [N, S, H, D] and k, v [N, S, Hkv, D] do not "
-              "match: ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
   const int64_t N = q.size(0), S = q.size(1), H = q.size(2), Hkv = k.size(2),
                 D = q.size(3);
-  TORCH_CHECK(Hkv >= 1 && H % Hkv == 0, "masked_attn: ", H,
-              " heads do not divide over ", Hkv, " key heads");
-  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0,
-              "masked_attn: head sizes are multiples of 8 up to 128, not ", D);
+  TORCH_CHECK_VALUE(Hkv >= 1 && H % Hkv == 0, "attention: ", H,
+                    " heads do not divide over ", Hkv, " key heads");
+  TORCH_CHECK_VALUE(D >= 8 && D <= 128 && D % 8 == 0,
+                    "attention: head sizes are multiples of 8 up to 128, not ",
+                    D);
   constexpr int64_t kMost = std::numeric_limits<int>::max();
-  TORCH_CHECK(S <= (1 << 22) && N <= kMost &&
-                  N * H * ((S + 63) / 64) <= kMost,
-              "masked_attn: too many tokens (a sequence has at most 2^22)");
-  TORCH_CHECK(scale > 0.0 && softcap >= 0.0,
-              "masked_attn: the scale must be positive, the cap not negative");
+  TORCH_CHECK_VALUE(
+      S <= (1 << 22) && N <= kMost && N * H * ((S + 63) / 64) <= kMost,
+      "attention: too many tokens (a sequence has at most 2^22)");
+  TORCH_CHECK_VALUE(scale > 0.0 && scale <= std::numeric_limits<float>::max(),
+                    "attention: the scale must be positive, got ", scale);
+  TORCH_CHECK_VALUE(
+      softcap >= 0.0 && softcap <= std::numeric_limits<float>::max(),
+      "attention: softcap must be finite and not negative, got ", softcap);
   MaskedAttn a{};
   a.N = static_cast<int>(N);
   a.S = static_cast<int>(S);
@@ -353,26 +363,29 @@ MaskedAttn describe(const torch::Tensor& q, const torch::Tensor& k,
   a.scale = static_cast<float>(scale);
   a.softcap = static_cast<float>(softcap);
   if (prefix.has_value()) {
-    check_gpu(*prefix, q.device(), "masked_attn: prefix");
-    TORCH_CHECK(prefix->scalar_type() == torch::kInt32 &&
-                    prefix->is_contiguous() && prefix->numel() == N,
-                "masked_attn: prefix must be int32 [", N, "]");
+    TORCH_CHECK_VALUE(causal,
+                      "attention: a prefix widens a causal mask: causal=True");
+    here(*prefix, "prefix");
+    TORCH_CHECK_VALUE(prefix->scalar_type() == torch::kInt32 &&
+                          prefix->dim() == 1 && prefix->size(0) == N &&
+                          prefix->is_contiguous(),
+                      "attention: prefix must be int32 [", N, "]");
     a.prefix = prefix->data_ptr<int>();
   }
   if (doc.has_value()) {
-    check_gpu(*doc, q.device(), "masked_attn: doc");
-    TORCH_CHECK(doc->scalar_type() == torch::kInt32 &&
-                    doc->is_contiguous() && doc->dim() == 2 &&
-                    doc->size(0) == N && doc->size(1) == S,
-                "masked_attn: doc must be contiguous int32 [", N, ", ", S,
-                "]");
+    here(*doc, "doc");
+    TORCH_CHECK_VALUE(doc->scalar_type() == torch::kInt32 &&
+                          doc->dim() == 2 && doc->size(0) == N &&
+                          doc->size(1) == S && doc->is_contiguous(),
+                      "attention: doc must be int32 [", N, ", ", S, "]");
     a.doc = doc->data_ptr<int>();
   }
   if (slopes.has_value()) {
-    check_gpu(*slopes, q.device(), "masked_attn: slopes");
-    TORCH_CHECK(slopes->scalar_type() == torch::kFloat32 &&
-                    slopes->is_contiguous() && slopes->numel() == H,
-                "masked_attn: slopes must be float32 [", H, "]");
+    here(*slopes, "slopes");
+    TORCH_CHECK_VALUE(slopes->scalar_type() == torch::kFloat32 &&
+                          slopes->dim() == 1 && slopes->size(0) == H &&
+                          slopes->is_contiguous(),
+                      "attention: slopes must be float32 [", H, "]");
     a.slopes = slopes->data_ptr<float>();
   }
   return a;
@@ -478,7 +491,7 @@ void masked_attn_bwd(torch::Tensor go, torch::Tensor q, torch::Tensor k,
 // ---- autograd -------------------------------------------------------------------
 // In C++: the engine's thread then needs no interpreter, which is most of a
 // small backward pass (norm of 4096 x 768, forward and backward: 115 us of
-// host time with functions in Python, BACKWARD here).
+// host time with functions in Python, 86 here).
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -633,20 +646,40 @@ struct MaskedAttnQKVFn : public torch::autograd::Function<MaskedAttnQKVFn> {
   }
 };
 
+// masks as the kernels read them
+struct Masks {
+  OptTensor prefix, doc, slopes;
+
+  Masks(const OptTensor& p, const OptTensor& d, const OptTensor& s) {
+    if (p.has_value()) prefix = p->contiguous();
+    if (d.has_value()) doc = d->contiguous();
+    if (s.has_value()) {
+      TORCH_CHECK_VALUE(!s->requires_grad(),
+                        "attention: slopes are constants: they get no "
+                        "gradient");
+      slopes = s->contiguous();
+    }
+  }
+};
+
 torch::Tensor masked_attention(torch::Tensor q, torch::Tensor k,
                                torch::Tensor v, double scale, bool causal,
                                double softcap, OptTensor prefix, OptTensor doc,
                                OptTensor slopes) {
-  return MaskedAttnFn::apply(q, k, v, scale, causal, softcap, prefix, doc,
-                             slopes);
+  const Masks m(prefix, doc, slopes);
+  return MaskedAttnFn::apply(q, k, v, scale, causal, softcap, m.prefix, m.doc,
+                             m.slopes);
 }
 
+// [N, S, H * D]
 torch::Tensor masked_attention_qkv(torch::Tensor qkv, double scale,
                                    bool causal, double softcap,
                                    OptTensor prefix, OptTensor doc,
                                    OptTensor slopes) {
-  return MaskedAttnQKVFn::apply(qkv, scale, causal, softcap, prefix, doc,
-                                slopes);
+  const Masks m(prefix, doc, slopes);
+  return MaskedAttnQKVFn::apply(qkv, scale, causal, softcap, m.prefix, m.doc,
+                                m.slopes)
+      .flatten(2);
 }
 
 }  // namespace
