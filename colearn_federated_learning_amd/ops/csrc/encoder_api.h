@@ -14,7 +14,7 @@ enum class Elem : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 constexpr int kAdamwTensors = 48;   // tensors a launch; the table is passed by
                                     // value and has to fit 4 KB of arguments
 constexpr int kAdamwBlock = 256;    // elements that share one 8-bit scale
-constexpr int kAdamwChunk = 2048;   // elements a workgroup
+constexpr int kAdamwChunk = 1024;   // elements a workgroup: a block a wave
 
 struct AdamwTensor {
   void* p;
