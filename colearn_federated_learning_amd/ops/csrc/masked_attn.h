@@ -72,7 +72,6 @@ typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(1))) const void global_void;
 
 template <typename T>
 DEV_INLINE f32x16 mfma(s16x8 a, s16x8 b, f32x16 c);
@@ -165,23 +164,32 @@ struct Stream {
   DEV_INLINE Stream(const short* p, int64_t stride) : base(p), ss(stride) {}
 
   // A tile of which every row is there and none is padding, and D == DP:
-  // straight from memory into LDS.  A wave's 16 bytes a lane land side by
-  // side, so the permutation of slots is in what a lane fetches.  No registers
-  // hold the tile on its way; the barrier before it is read waits for it.
+  // straight from memory into LDS, no registers on the way.  A wave's 16 bytes
+  // a lane land side by side, so the permutation of slots is in what a lane
+  // fetches.  In assembly, which the compiler does not look into: it takes a
+  // load into LDS for a write that every later read of LDS may depend on, and
+  // would wait for the next tile in the middle of this one.  What has to wait
+  // is `arrived`, before the barrier that hands the tile over.
   DEV_INLINE void send(char* lds, int t0) const {
     const int row = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
     const unsigned step = static_cast<unsigned>(2 * ss);
     // the permutation goes by the row's lowest three bits, which all passes
     // share: kStep is a multiple of 8
-    const unsigned off =
-        row * step + ((L::at(row, slot) - row * (DP * 2)));
+    const unsigned off = row * step + (L::at(row, slot) - row * (DP * 2));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const char* p = reinterpret_cast<const char*>(base + t0 * ss);
+    const unsigned to = __builtin_amdgcn_readfirstlane(
+        static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)lds)) +
+        wave * 1024);
 #pragma unroll
     for (int i = 0; i < L::kPer; ++i)
-      __builtin_amdgcn_global_load_lds(
-          (global_void*)(p + off + i * L::kStep * step),
-          (lds_void*)(lds + i * 4096 + wave * 1024), 16, 0, 0);
+      asm volatile(
+          "s_mov_b32 m0, %0\n\t"
+          "s_nop 0\n\t"
+          "global_load_lds_dwordx4 %1, %2"
+          :
+          : "s"(to + i * 4096), "v"(off), "s"(p + i * L::kStep * step)
+          : "memory", "m0");
   }
   // Any tile: rows that `live` has no bit of, and columns past D, as zeros.
   DEV_INLINE void copy(char* lds, int t0, int S, int D,
@@ -199,6 +207,9 @@ struct Stream {
     }
   }
 };
+
+// Everything that this wave has sent is in LDS.
+DEV_INLINE void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // The streamed tokens' documents: every wave's lanes hold those of the tile's
 // 64 tokens.
@@ -235,6 +246,15 @@ DEV_INLINE void own_rows(const short* row, bool live, int D,
     r[kk] = live && col < D ? *reinterpret_cast<const s16x8*>(row + col)
                             : zero;
   }
+}
+
+// The operand is in its registers from here on.  Before a loop: loads that may
+// still be under way when it begins would be waited for, with everything sent
+// since, in each of its rounds.
+template <int N>
+DEV_INLINE void settle(s16x8 (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(r[i]));
 }
 
 // a transposed result: this lane's token gets columns 32 db + (r & 3) +

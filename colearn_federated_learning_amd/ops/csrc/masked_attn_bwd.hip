@@ -85,6 +85,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
     unsigned next = entry_of(sm.list, 1, count);
     fetch(0, entry);
     keep(0, entry);
+    settle(qf);
+    settle(gf);
+    asm volatile("" : "+v"(lse));
+    arrived();
     __syncthreads();
     for (int e = 0; e < count; ++e) {
       const int buf = e & 1;
@@ -132,6 +136,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
       if (e + 1 < count) keep(buf ^ 1, next);
       entry = next;
       next = __builtin_amdgcn_readfirstlane(after);
+      arrived();
       __syncthreads();
     }
   }
@@ -277,6 +282,9 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       unsigned next = entry_of(sm.list, 1, count);
       fetch(0, entry);
       keep(0, entry);
+      settle(kf);
+      settle(vf);
+      arrived();
       __syncthreads();
       for (int e = 0; e < count; ++e) {
         const int buf = e & 1;
@@ -293,6 +301,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
         if (e + 1 < count) keep(buf ^ 1, next);
         entry = next;
         next = __builtin_amdgcn_readfirstlane(after);
+        arrived();
         __syncthreads();
       }
     }

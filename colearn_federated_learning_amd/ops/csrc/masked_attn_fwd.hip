@@ -118,6 +118,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
     unsigned next = entry_of(sm.list, 1, count);
     fetch(0, entry);
     keep(0, entry);
+    settle(qf);
+    arrived();
     __syncthreads();
     for (int e = 0; e < count; ++e) {
       const int buf = e & 1;
@@ -139,6 +141,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
       if (e + 1 < count) keep(buf ^ 1, next);
       entry = next;
       next = __builtin_amdgcn_readfirstlane(after);
+      arrived();
       __syncthreads();
     }
   }
