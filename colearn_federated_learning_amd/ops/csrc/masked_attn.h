@@ -115,9 +115,10 @@ DEV_INLINE float fast_tanh(float x) {
 DEV_INLINE float other_half(float x) { return swap32(x); }
 
 // A tile of kTile rows of DP 16-bit values.  16-byte slots are permuted
-// within a row so that neither read below hits a bank twice: eight
-// consecutive rows of a slot (row operand) lie over all slots of 128 bytes,
-// and so do four consecutive rows of two slots (transposed operand).
+// within a row so that neither read below hits a bank twice in 256 bytes: 16
+// consecutive rows of one slot (row operand) lie over all of them, and so do
+// four consecutive rows of four neighbouring slots (transposed operand, 32
+// lanes).
 template <int DP>
 struct Tile {
   static constexpr int kSlots = DP / 8;
@@ -126,8 +127,10 @@ struct Tile {
   static constexpr int kBytes = kTile * DP * 2;
 
   DEV_INLINE static int at(int row, int slot) {
-    const int f = DP == 32 ? ((row & 2) | ((row >> 2) & 1))
-                           : (((row & 3) << 1) | ((row >> 2) & 1));
+    const int f = DP == 32   ? (row >> 2) & 3
+                  : DP == 64 ? (((row & 3) << 1) | ((row >> 2) & 1)) ^
+                                   (((row >> 3) & 1) << 1)
+                             : ((row & 3) << 2) | ((row >> 2) & 3);
     return row * (DP * 2) + ((slot ^ f) << 4);
   }
 
@@ -144,10 +147,11 @@ struct Tile {
     const int i = lane & 15;
     const int row = ((lane >> 5) << 2) + (i >> 2);
     const int slot = db * 4 + ((lane >> 4) & 1) * 2 + ((i >> 1) & 1);
-    const char* p = half + at(row, slot) + (i & 1) * 8 + ks * (16 * DP * 2);
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const char* p = half + (i & 1) * 8 + ks * (16 * DP * 2);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(p + at(row, slot)));
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4*)(p + 8 * DP * 2));
+        (lds_s16x4*)(p + at(row + 8, slot)));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
@@ -173,8 +177,8 @@ struct Stream {
   DEV_INLINE void send(char* lds, int t0) const {
     const int row = threadIdx.x / L::kSlots, slot = threadIdx.x % L::kSlots;
     const unsigned step = static_cast<unsigned>(2 * ss);
-    // the permutation goes by the row's lowest three bits, which all passes
-    // share: kStep is a multiple of 8
+    // the permutation goes by the row's lowest four bits, which all passes
+    // share: kStep is a multiple of 16
     const unsigned off = row * step + (L::at(row, slot) - row * (DP * 2));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const char* p = reinterpret_cast<const char*>(base + t0 * ss);
