@@ -441,17 +441,40 @@ struct Score {
                                                : 0.f;
   }
 
-  // dist: owned token minus the streamed token of register 0
-  DEV_INLINE void shape(f32x16& z, float dist) const {
+  DEV_INLINE void bend(f32x16& z) const {
     if constexpr (M == kCap) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) z[r] = fast_tanh(z[r] * cap_in);
     }
+  }
+  // dist: owned token minus the streamed token of register 0
+  DEV_INLINE void shape(f32x16& z, float dist) const {
+    bend(z);
     if constexpr (M != kPlain) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         z[r] -= slope * fabsf(dist - ((r & 3) + 8 * (r >> 2)));
     }
+  }
+  // The same but for a part that all of the lane's scores share, which is
+  // returned.  rel: the wave's first owned token minus the first streamed one.
+  // Where one side's tokens all precede the other's, the distance is a sum of
+  // the lane's part and the register's, one operation a score.
+  DEV_INLINE float shape(f32x16& z, float dist, int rel) const {
+    if constexpr (M == kPlain) return 0.f;
+    bend(z);
+    if (rel > -31 && rel < 31) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        z[r] -= slope * fabsf(dist - ((r & 3) + 8 * (r >> 2)));
+      return 0.f;
+    }
+    const float s = rel > 0 ? slope : -slope;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      z[r] = __builtin_fmaf(static_cast<float>((r & 3) + 8 * (r >> 2)), s,
+                            z[r]);
+    return -s * dist;
   }
 };
 

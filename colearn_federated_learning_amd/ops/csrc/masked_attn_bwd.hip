@@ -21,7 +21,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
-  const int own = own0 + (wave / KS) * 32 + (lane & 31);
+  const int own_wave = own0 + (wave / KS) * 32;
+  const int own = own_wave + (lane & 31);
   const int found = doc_of(a, n, own);
   const bool live = found >= 0;
   const int own_doc = live ? found : -2;
@@ -119,12 +120,14 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
             dp[r] *= 1.f - th * th;
           }
         }
-        sc.shape(z, static_cast<float>(own - t0 - other));
+        const float lane_part =
+            sc.c * sc.shape(z, static_cast<float>(own - t0 - other),
+                            own_wave - t0 - kb * 32);
         if (c == 1)
           mask<true>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          dp[r] *= fast_exp2(__builtin_fmaf(z[r], sc.c, -lse));
+          dp[r] *= fast_exp2(__builtin_fmaf(z[r], sc.c, lane_part - lse));
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const s16x8 x = round8<T>(dp, s);

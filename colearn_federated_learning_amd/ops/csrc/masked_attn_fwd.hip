@@ -27,6 +27,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
     MaskedAttn a) {
   using L = Tile<DP>;
   constexpr int OWN = 128 / KS;
+  // Both halves of a tile at once where registers allow it: one's products run
+  // under the other's exponentials.  Size 64, 1 x 8192 tokens: 255 us, one
+  // after the other 264; size 128: 555 and 552.
+  constexpr bool kJoint = KS == 1 && DP <= 64;
   __shared__ __align__(16) Smem<DP> sm;
   int n, h, own0;
   locate<OWN>(a, a.H, a.causal, &n, &h, &own0);
@@ -34,7 +38,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
-  const int own = own0 + (wave / KS) * 32 + (lane & 31);
+  const int own_wave = own0 + (wave / KS) * 32;
+  const int own = own_wave + (lane & 31);
   const int found = doc_of(a, n, own);
   const bool live = found >= 0;
   const int own_doc = live ? found : -2;
@@ -51,20 +56,32 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
   for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
   float m = -INFINITY, l = 0.f;  // m: of c z; l: this half's share
 
-  // 32 streamed keys from t0 on; mixed: some pairs of them are not attended
-  auto work = [&](const char* kt, const char* vt, const int* dt, int t0,
-                  bool mixed) {
-    f32x16 z = 0.f;
+  // N x 32 streamed keys from t0 on; cls: their marks, two bits each
+  auto work = [&](auto count, const char* kt, const char* vt, const int* dt,
+                  int t0, unsigned cls) {
+    constexpr int N = decltype(count)::value;
+    f32x16 z[N];
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
-      z = mfma<T>(L::rows(kt, kk), qf[kk], z);
-    const int other = t0 + 4 * half;
-    sc.shape(z, static_cast<float>(own - other));
-    if (mixed) mask<true>(z, own_doc, lim, other, dt + 4 * half);
-    float mx = z[0];
+    for (int i = 0; i < N; ++i) {
+      z[i] = 0.f;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, z[r]);
-    mx *= sc.c;
+      for (int kk = 0; kk < DP / 16; ++kk)
+        z[i] = mfma<T>(L::rows(kt + i * (L::kBytes / 2), kk), qf[kk], z[i]);
+    }
+    float mx = -INFINITY, lane_part[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int other = t0 + i * 32 + 4 * half;
+      lane_part[i] = sc.c * sc.shape(z[i], static_cast<float>(own - other),
+                                     own_wave - t0 - i * 32);
+      // a half without any pair comes along as one whose pairs are all masked
+      if (((cls >> (2 * i)) & 3) != 2)
+        mask<true>(z[i], own_doc, lim, other, dt + i * 32 + 4 * half);
+      float hi = z[i][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) hi = fmaxf(hi, z[i][r]);
+      mx = fmaxf(mx, __builtin_fmaf(hi, sc.c, lane_part[i]));
+    }
     // The sums are kept relative to a maximum that may be outgrown by 2^8
     // before they are scaled anew: p stays within both types' range, and its
     // rounding is relative.
@@ -79,16 +96,21 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
     }
     const float top = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -top));
-      l += z[r];
-    }
+    for (int i = 0; i < N; ++i) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const s16x8 p = round8<T>(z, s);
+      for (int r = 0; r < 16; ++r) {
+        z[i][r] =
+            fast_exp2(__builtin_fmaf(z[i][r], sc.c, lane_part[i] - top));
+        l += z[i][r];
+      }
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db)
-        acc[db] = mfma<T>(L::cols(vt, s, db), p, acc[db]);
+      for (int s = 0; s < 2; ++s) {
+        const s16x8 p = round8<T>(z[i], s);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+          acc[db] =
+              mfma<T>(L::cols(vt + i * (L::kBytes / 2), s, db), p, acc[db]);
+      }
     }
   };
   const int tiles = (a.S + kTile - 1) / kTile;
@@ -130,13 +152,19 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
       const char* vt = sm.tile[buf][1];
       const int* dt = sm.doc[buf];
       const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
+      if constexpr (kJoint) {
+        if (cls != 0)
+          work(std::integral_constant<int, 2>(), kt, vt, dt, t0, cls);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2 / KS; ++i) {
-        const int hf = KS == 2 ? part : i;
-        const unsigned c = (cls >> (2 * hf)) & 3;
-        if (c != 0)
-          work(kt + hf * (L::kBytes / 2), vt + hf * (L::kBytes / 2),
-               dt + hf * 32, t0 + hf * 32, c == 1);
+        for (int i = 0; i < 2 / KS; ++i) {
+          const int hf = KS == 2 ? part : i;
+          const unsigned c = (cls >> (2 * hf)) & 3;
+          if (c != 0)
+            work(std::integral_constant<int, 1>(),
+                 kt + hf * (L::kBytes / 2), vt + hf * (L::kBytes / 2),
+                 dt + hf * 32, t0 + hf * 32, c);
+        }
       }
       if (e + 1 < count) keep(buf ^ 1, next);
       entry = next;
