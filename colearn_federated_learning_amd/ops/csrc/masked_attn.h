@@ -238,17 +238,25 @@ struct Docs {
   }
 };
 
-// right operand of an owned token's row: columns 16 kk + 8 h + 0..7
+// right operand of an owned token's row: columns 16 kk + 8 h + 0..7.  The load
+// does not wait to know whether the token is there or padding (`row` is one
+// that can be read); `clear` makes zeros of those and of columns past D.
 template <int DP>
-DEV_INLINE void own_rows(const short* row, bool live, int D,
-                         s16x8 (&r)[DP / 16]) {
+DEV_INLINE void own_rows(const short* row, int D, s16x8 (&r)[DP / 16]) {
   const int h = (threadIdx.x % kWave) >> 5;
 #pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk)
+    r[kk] =
+        *reinterpret_cast<const s16x8*>(row + min(kk * 16 + h * 8, D - 8));
+}
+template <int DP>
+DEV_INLINE void clear(bool live, int D, s16x8 (&r)[DP / 16]) {
+  const int h = (threadIdx.x % kWave) >> 5;
+  if (D == DP && __all(live)) return;
+#pragma unroll
   for (int kk = 0; kk < DP / 16; ++kk) {
-    const int col = kk * 16 + h * 8;
     const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-    r[kk] = live && col < D ? *reinterpret_cast<const s16x8*>(row + col)
-                            : zero;
+    if (!live || kk * 16 + h * 8 >= D) r[kk] = zero;
   }
 }
 
@@ -261,11 +269,11 @@ DEV_INLINE void settle(s16x8 (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(r[i]));
 }
 
-// a transposed result: this lane's token gets columns 32 db + (r & 3) +
-// 8 (r >> 2) + 4 h
-template <typename T, int DP>
-DEV_INLINE void store_cols(T* row, const f32x16 (&acc)[DP / 32], float f,
-                           bool live, int D) {
+// A transposed result: this lane's token has columns 32 db + (r & 3) +
+// 8 (r >> 2) + 4 h, times f, or zeros.
+template <int DP>
+DEV_INLINE void put_cols(float* row, const f32x16 (&acc)[DP / 32], float f,
+                         bool live, int D) {
   const int h = (threadIdx.x % kWave) >> 5;
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db)
@@ -277,6 +285,37 @@ DEV_INLINE void store_cols(T* row, const f32x16 (&acc)[DP / 32], float f,
       for (int j = 0; j < 4; ++j) x[j] = live ? acc[db][g * 4 + j] * f : 0.f;
       if (col < D) elem_store4(row + col, x);
     }
+}
+// The same for a wave's 32 tokens from `first` on, rounded to T, by way of LDS:
+// a lane's own stores would be 8 bytes each, a row apart; these are whole rows,
+// 16 bytes a lane.  lds: 64 DP bytes that nobody but this wave touches.
+template <typename T, int DP>
+DEV_INLINE void store_cols(char* lds, T* base, int64_t ss, int first, int S,
+                           const f32x16 (&acc)[DP / 32], float f, bool live,
+                           int D) {
+  using L = Tile<DP>;
+  const int lane = threadIdx.x % kWave, h = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = live ? acc[db][g * 4 + j] * f : 0.f;
+      elem_store4(reinterpret_cast<T*>(lds + L::at(lane & 31, db * 4 + g) +
+                                       h * 8),
+                  x);
+    }
+  const int slot = lane % L::kSlots;
+#pragma unroll
+  for (int i = 0; i < L::kSlots / 2; ++i) {
+    const int row = i * (kWave / L::kSlots) + lane / L::kSlots;
+    const s16x8 x =
+        *reinterpret_cast<const s16x8*>(lds + L::at(row, slot));
+    if (first + row < S && slot * 8 < D)
+      *reinterpret_cast<s16x8*>(reinterpret_cast<short*>(base) +
+                                (first + row) * ss + slot * 8) = x;
+  }
 }
 
 // What the pairs of tokens [q0, q1) x [k0, k1) are: 0 none attended, 1 some,

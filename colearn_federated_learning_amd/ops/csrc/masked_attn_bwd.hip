@@ -32,13 +32,17 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
   const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss);
   const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss);
   s16x8 qf[DP / 16], gf[DP / 16];
-  own_rows<DP>(row_of(a.q, n, h) + own * a.q.ss, live, a.D, qf);
-  own_rows<DP>(row_of(a.go, n, h) + own * a.go.ss, live, a.D, gf);
+  const int there = min(own, a.S - 1);
+  own_rows<DP>(row_of(a.q, n, h) + there * a.q.ss, a.D, qf);
+  own_rows<DP>(row_of(a.go, n, h) + there * a.go.ss, a.D, gf);
   float delta = 0.f, lse = INFINITY;
   {
     const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S + own;
     s16x8 of[DP / 16];
-    own_rows<DP>(row_of(a.o, n, h) + own * a.o.ss, live, a.D, of);
+    own_rows<DP>(row_of(a.o, n, h) + there * a.o.ss, a.D, of);
+    clear<DP>(live, a.D, qf);
+    clear<DP>(live, a.D, gf);
+    clear<DP>(live, a.D, of);
     typedef __attribute__((ext_vector_type(8))) typename Bits16<T>::hw V;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
@@ -59,6 +63,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
 
+  settle(qf);
+  settle(gf);
+  asm volatile("" : "+v"(lse));
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
     const int count = list_tiles<true, OWN / 32>(a, n, own0, base, sum,
@@ -86,9 +93,6 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
     unsigned next = entry_of(sm.list, 1, count);
     fetch(0, entry);
     keep(0, entry);
-    settle(qf);
-    settle(gf);
-    asm volatile("" : "+v"(lse));
     arrived();
     __syncthreads();
     for (int e = 0; e < count; ++e) {
@@ -143,9 +147,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
       __syncthreads();
     }
   }
+  // of the tile buffers: this wave's own part, or its pair's
+  char* const mine =
+      &sm.tile[0][0][0] +
+      (KS == 2 ? (wave / 2) * (DP / 2) * kWave * 4 : wave * DP * kWave);
   if constexpr (KS == 2) {
-    float* at = reinterpret_cast<float*>(&sm.tile[0][0][0]) +
-                (wave / 2) * (DP / 2) * kWave;
+    float* at = reinterpret_cast<float*>(mine);
     __syncthreads();
     if (part == 1) leave(at, acc);
     __syncthreads();
@@ -155,10 +162,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) acc[i] += o[i];
   }
-  if (own < a.S)
-    store_cols<T, DP>(static_cast<T*>(a.gq.p) + n * a.gq.sn + own * a.gq.ss +
-                          h * a.gq.sh,
-                      acc, a.scale, live, a.D);
+  store_cols<T, DP>(mine,
+                    static_cast<T*>(a.gq.p) + n * a.gq.sn + h * a.gq.sh,
+                    a.gq.ss, own_wave, a.S, acc, a.scale, live, a.D);
 }
 
 template <typename T, int DP, Mode M, int KS>
@@ -175,7 +181,8 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
-  const int own = own0 + (wave / KS) * 32 + (lane & 31);
+  const int own_wave = own0 + (wave / KS) * 32;
+  const int own = own_wave + (lane & 31);
   const int found = doc_of(a, n, own);
   const bool live = found >= 0;
   const int own_doc = live ? found : -2;
@@ -183,8 +190,9 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   Docs docs(a, n);
   const int4* sum = summary_of(a, n, sm.sum);
   s16x8 kf[DP / 16], vf[DP / 16];
-  own_rows<DP>(row_of(a.k, n, hk) + own * a.k.ss, live, a.D, kf);
-  own_rows<DP>(row_of(a.v, n, hk) + own * a.v.ss, live, a.D, vf);
+  const int there = min(own, a.S - 1);
+  own_rows<DP>(row_of(a.k, n, hk) + there * a.k.ss, a.D, kf);
+  own_rows<DP>(row_of(a.v, n, hk) + there * a.v.ss, a.D, vf);
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = 0.f;
@@ -243,6 +251,10 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       }
     }
   };
+  clear<DP>(live, a.D, kf);
+  clear<DP>(live, a.D, vf);
+  settle(kf);
+  settle(vf);
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
     const int count = list_tiles<false, OWN / 32>(a, n, own0, base, sum,
@@ -285,9 +297,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       unsigned next = entry_of(sm.list, 1, count);
       fetch(0, entry);
       keep(0, entry);
-      settle(kf);
-      settle(vf);
-      arrived();
+          arrived();
       __syncthreads();
       for (int e = 0; e < count; ++e) {
         const int buf = e & 1;
@@ -309,9 +319,10 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       }
     }
   }
+  char* const mine = &sm.tile[0][0][0] +
+                     (KS == 2 ? (wave / 2) * DP * kWave * 4 : wave * DP * kWave);
   if constexpr (KS == 2) {
-    float* at = reinterpret_cast<float*>(&sm.tile[0][0][0]) +
-                (wave / 2) * DP * kWave;
+    float* at = reinterpret_cast<float*>(mine);
     __syncthreads();
     if (part == 1) {
       leave(at, dk);
@@ -327,21 +338,21 @@ masked_attn_dkv_kernel(MaskedAttn a) {
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dv[i] += o[i];
   }
-  if (own < a.S && a.shares > 1) {
+  if (a.shares > 1) {
+    if (own >= a.S) return;
     const int64_t size = static_cast<int64_t>(a.N) * a.S * a.Hkv * a.D;
     float* at = a.partial + share * size +
                 ((static_cast<int64_t>(n) * a.S + own) * a.Hkv + hk) * a.D;
-    store_cols<float, DP>(at, dk, a.scale, live, a.D);
-    store_cols<float, DP>(at + a.shares * size, dv, 1.f / kLift<T>, live,
-                          a.D);
-  } else if (own < a.S) {
-    store_cols<T, DP>(static_cast<T*>(a.gk.p) + n * a.gk.sn + own * a.gk.ss +
-                          hk * a.gk.sh,
-                      dk, a.scale, live, a.D);
-    store_cols<T, DP>(static_cast<T*>(a.gv.p) + n * a.gv.sn + own * a.gv.ss +
-                          hk * a.gv.sh,
-                      dv, 1.f / kLift<T>, live, a.D);
+    put_cols<DP>(at, dk, a.scale, live, a.D);
+    put_cols<DP>(at + a.shares * size, dv, 1.f / kLift<T>, live, a.D);
+    return;
   }
+  store_cols<T, DP>(mine,
+                    static_cast<T*>(a.gk.p) + n * a.gk.sn + hk * a.gk.sh,
+                    a.gk.ss, own_wave, a.S, dk, a.scale, live, a.D);
+  store_cols<T, DP>(mine,
+                    static_cast<T*>(a.gv.p) + n * a.gv.sn + hk * a.gv.sh,
+                    a.gv.ss, own_wave, a.S, dv, 1.f / kLift<T>, live, a.D);
 }
 
 // Shares' sums, four elements a thread: grid.y 0 dk, 1 dv.

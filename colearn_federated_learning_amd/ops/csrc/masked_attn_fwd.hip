@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
   const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss);
   const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss);
   s16x8 qf[DP / 16];
-  own_rows<DP>(row_of(a.q, n, h) + own * a.q.ss, live, a.D, qf);
+  own_rows<DP>(row_of(a.q, n, h) + min(own, a.S - 1) * a.q.ss, a.D, qf);
   const Score<M> sc(a, h);
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -113,6 +113,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
       }
     }
   };
+  clear<DP>(live, a.D, qf);
+  settle(qf);
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
     const int count = list_tiles<true, OWN / 32>(a, n, own0, base, sum,
@@ -140,7 +142,6 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
     unsigned next = entry_of(sm.list, 1, count);
     fetch(0, entry);
     keep(0, entry);
-    settle(qf);
     arrived();
     __syncthreads();
     for (int e = 0; e < count; ++e) {
@@ -174,10 +175,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
     }
   }
   l += other_half(l);
+  constexpr int N = DP / 32;
+  // of the tile buffers: this wave's own part, or its pair's
+  char* const mine = &sm.tile[0][0][0] +
+                     (KS == 2 ? (wave / 2) * (N * 16 + 2) * kWave * 4
+                              : wave * DP * kWave);
   if constexpr (KS == 2) {
-    constexpr int N = DP / 32;
-    float* at = reinterpret_cast<float*>(&sm.tile[0][0][0]) +
-                (wave / 2) * (N * 16 + 2) * kWave;
+    float* at = reinterpret_cast<float*>(mine);
     __syncthreads();  // every list may have been empty
     if (part == 1) {
       leave(at, acc);
@@ -198,15 +202,14 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = acc[i] * f + o[i] * f2;
   }
-  if (own < a.S) {
-    T* o = static_cast<T*>(a.o.p) + n * a.o.sn + own * a.o.ss + h * a.o.sh;
-    // NaN in a live row's sum is kept: only an empty row is cleared
-    const bool clear = !live || l == 0.f;
-    store_cols<T, DP>(o, acc, clear ? 0.f : 1.f / l, !clear, a.D);
-    if (half == 0)
-      a.lse[(static_cast<int64_t>(n) * a.H + h) * a.S + own] =
-          clear ? INFINITY : m + log2f(l);
-  }
+  // NaN in a live row's sum is kept: only an empty row is cleared
+  const bool empty = !live || l == 0.f;
+  store_cols<T, DP>(mine,
+                    static_cast<T*>(a.o.p) + n * a.o.sn + h * a.o.sh, a.o.ss,
+                    own_wave, a.S, acc, empty ? 0.f : 1.f / l, !empty, a.D);
+  if (own < a.S && half == 0)
+    a.lse[(static_cast<int64_t>(n) * a.H + h) * a.S + own] =
+        empty ? INFINITY : m + log2f(l);
 }
 
 struct Forward {
