@@ -49,6 +49,17 @@ class ModelConfig:
     num_layers: Optional[int] = None
     num_heads: Optional[int] = None
     intermediate_size: Optional[int] = None
+    # bert_base attention beyond rows of one text each (models/bert.py):
+    # a token that ends a document within a row, one that pads, a cap on the
+    # scores, a bias by distance.  They take no dropout of probabilities:
+    # set attn_dropout=0 with them (None => dropout).
+    doc_sep_token: Optional[int] = None
+    pad_token: Optional[int] = None
+    attn_softcap: float = 0.0
+    attn_distance_bias: bool = False
+    attn_dropout: Optional[float] = None
+    # residual add and LayerNorm in one kernel (bert_base)
+    fused_add_norm: bool = False
 
 
 @dataclass
@@ -58,7 +69,7 @@ class TrainingConfig:
     lr: float = 0.05
     momentum: float = 0.9
     weight_decay: float = 0.0
-    optimizer: str = "sgd"  # sgd | adam
+    optimizer: str = "sgd"  # sgd | adam | adamw | adamw8 (8-bit states)
     dtype: str = "float32"  # float32 | bfloat16 (autocast compute dtype)
     # FedProx proximal term strength (0 => plain FedAvg local objective)
     fedprox_mu: float = 0.0

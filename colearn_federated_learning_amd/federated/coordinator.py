@@ -71,6 +71,8 @@ class FederatedServer:
         self.optimizer = make_flat_optimizer(
             cfg.train.optimizer, self.flat.flat_w, self.flat.flat_g,
             cfg.train, flat_ref=self.global_flat,
+            segments=[(n, len(shape) > 1) for n, shape in
+                      zip(self.flat.numels, self.flat.shapes)],
         )
         self.aggregator = Aggregator(cfg.agg, self.device)
         self.sampler = ClientSampler(

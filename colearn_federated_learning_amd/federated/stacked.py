@@ -249,6 +249,10 @@ class StackedEngine:
         self.optimizer = make_flat_optimizer(
             cfg.train.optimizer, self.sflat.flat_w, self.sflat.flat_g,
             cfg.train, flat_ref=self.flat_ref,
+            # every client's tensor is one of its own
+            segments=[(n, len(shape) > 1) for n, shape in
+                      zip(self.sflat.t_numels, self.sflat.t_shapes)
+                      for _ in range(self.G)],
         )
         # stacked DP: per-sample grads for ALL clients' samples in one
         # backward (hook engine over the stacked modules), clip + per-

@@ -5,22 +5,24 @@ Post-LN transformer encoder (BERT architecture: 12 layers, hidden 768,
 route through ops.gemm (MFMA bf16 GEMM on gfx950), attention score/context
 matmuls through ops.gemm.colearn_matmul, LayerNorms through ops.norms.
 At the mandated seq_len=128 attention is two small batched GEMMs + a
-softmax — no flash/long-context machinery is warranted (SURVEY.md §5,
-long-context entry: explicitly out of scope).
+softmax.  Rows that hold several documents or padding, capped scores and
+distance biases (BertConfig) run through ops.attention.colearn_attention,
+which serves any length.
 """
 
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.attention import colearn_attention_qkv, distance_slopes
 from ..ops.gemm import colearn_linear, colearn_matmul, colearn_matmul_nt
-from ..ops.norms import ColearnLayerNorm
+from ..ops.norms import ColearnLayerNorm, colearn_add_layer_norm
 from .base import ColearnModel
 
 
@@ -34,8 +36,32 @@ class BertConfig:
     max_position_embeddings: int = 512
     dropout: float = 0.1
     layer_norm_eps: float = 1e-12
+    # a token that ends a document: tokens attend within their document only
+    doc_sep_token: Optional[int] = None
+    # padding: attends to nothing and is attended by nothing
+    pad_token: Optional[int] = None
+    attn_softcap: float = 0.0         # 0: scores are not capped
+    attn_distance_bias: bool = False  # ops.attention.distance_slopes
+    attn_dropout: Optional[float] = None  # of probabilities; None: dropout
+    fused_add_norm: bool = False      # residual add + norm in one kernel
+
+    @property
+    def masked_attention(self) -> bool:
+        """Whether attention runs through ops.attention.colearn_attention."""
+        return (self.doc_sep_token is not None or self.pad_token is not None
+                or self.attn_softcap != 0.0 or self.attn_distance_bias)
+
+    @property
+    def probs_dropout(self) -> float:
+        return (self.dropout if self.attn_dropout is None
+                else self.attn_dropout)
 
     def __post_init__(self) -> None:
+        if self.masked_attention and self.probs_dropout != 0.0:
+            raise ValueError(
+                "attention with documents, padding, a cap or a distance bias "
+                "has no dropout of its probabilities: set attn_dropout=0 "
+                f"(it is {self.probs_dropout})")
         if self.hidden_size % self.num_heads:
             raise ValueError(
                 f"hidden_size {self.hidden_size} must be divisible by "
@@ -53,18 +79,57 @@ class _Linear(nn.Module):
         return colearn_linear(x, self.weight, self.bias)
 
 
-class BertSelfAttention(nn.Module):
+def document_ids(ids: torch.Tensor, cfg: BertConfig
+                 ) -> Optional[torch.Tensor]:
+    """int32 document of every token, -1 for padding; None if the config
+    tells neither apart.  A separator belongs to the document that it ends."""
+    if cfg.doc_sep_token is None and cfg.pad_token is None:
+        return None
+    if cfg.doc_sep_token is None:
+        doc = torch.zeros_like(ids, dtype=torch.int32)
+    else:
+        ends = ids.eq(cfg.doc_sep_token).to(torch.int32)
+        doc = ends.cumsum(dim=1, dtype=torch.int32) - ends
+    if cfg.pad_token is not None:
+        doc = doc.masked_fill(ids.eq(cfg.pad_token), -1)
+    return doc
+
+
+class MaskedAttentionMixin:
+    """What the sequential and the stacked attention share of the config."""
+
+    def _init_masked(self, cfg: BertConfig) -> None:
+        self.masked = cfg.masked_attention
+        self.softcap = cfg.attn_softcap
+        self.distance_bias = cfg.attn_distance_bias
+        self._slopes = None  # a constant, made where it is first used
+
+    def _masked_attention(self, qkv: torch.Tensor, doc) -> torch.Tensor:
+        """[b, s, 3, h, dh] -> [b, s, h * dh]"""
+        slopes = None
+        if self.distance_bias:
+            if self._slopes is None or self._slopes.device != qkv.device:
+                self._slopes = distance_slopes(self.h, qkv.device)
+            slopes = self._slopes
+        return colearn_attention_qkv(qkv, doc=doc, softcap=self.softcap,
+                                     slopes=slopes)
+
+
+class BertSelfAttention(nn.Module, MaskedAttentionMixin):
     def __init__(self, cfg: BertConfig) -> None:
         super().__init__()
+        self._init_masked(cfg)
         self.h = cfg.num_heads
         self.dh = cfg.hidden_size // cfg.num_heads
         self.qkv = _Linear(cfg.hidden_size, 3 * cfg.hidden_size)
         self.out = _Linear(cfg.hidden_size, cfg.hidden_size)
-        self.drop = nn.Dropout(cfg.dropout)
+        self.drop = nn.Dropout(cfg.probs_dropout)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, doc=None) -> torch.Tensor:
         b, s, d = x.shape
         qkv = self.qkv(x).view(b, s, 3, self.h, self.dh)
+        if self.masked:
+            return self.out(self._masked_attention(qkv, doc))
         q, k, v = (
             qkv[:, :, i].transpose(1, 2).reshape(b * self.h, s, self.dh)
             for i in range(3)
@@ -86,10 +151,19 @@ class BertLayer(nn.Module):
         self.fc2 = _Linear(cfg.intermediate_size, cfg.hidden_size)
         self.ln2 = ColearnLayerNorm(cfg.hidden_size, cfg.layer_norm_eps)
         self.drop = nn.Dropout(cfg.dropout)
+        self.fused_add_norm = cfg.fused_add_norm
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x = self.ln1(x + self.drop(self.attn(x)))
-        x = self.ln2(x + self.drop(self.fc2(F.gelu(self.fc1(x)))))
+    def _join(self, ln: ColearnLayerNorm, x: torch.Tensor,
+              branch: torch.Tensor) -> torch.Tensor:
+        if self.fused_add_norm:
+            return colearn_add_layer_norm(branch, x, ln.weight, ln.bias,
+                                          ln.eps)[0]
+        return ln(x + branch)
+
+    def forward(self, x: torch.Tensor, doc=None) -> torch.Tensor:
+        x = self._join(self.ln1, x, self.drop(self.attn(x, doc)))
+        x = self._join(self.ln2, x,
+                       self.drop(self.fc2(F.gelu(self.fc1(x)))))
         return x
 
 
@@ -117,8 +191,9 @@ class BertForMaskedLM(ColearnModel):
         pos = torch.arange(s, device=ids.device)
         x = self.tok_emb(ids) + self.pos_emb(pos)[None]
         x = self.drop(self.emb_ln(x))
+        doc = document_ids(ids, self.cfg)
         for layer in self.layers:
-            x = layer(x)
+            x = layer(x, doc)
         return x
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:

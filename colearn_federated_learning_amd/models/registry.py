@@ -50,6 +50,9 @@ def bert_config(model_cfg: ModelConfig, data_cfg: DataConfig):
         max_position_embeddings=max(data_cfg.seq_len, 512),
         dropout=model_cfg.dropout,
     )
+    for f in ("doc_sep_token", "pad_token", "attn_softcap",
+              "attn_distance_bias", "attn_dropout", "fused_add_norm"):
+        kw[f] = getattr(model_cfg, f)
     for f in ("hidden_size", "num_layers", "num_heads", "intermediate_size"):
         v = getattr(model_cfg, f)
         if v is not None:

@@ -27,11 +27,12 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops import native_enabled
 from ..ops.elemwise import colearn_gelu
 from ..ops.gemm import colearn_matmul, colearn_matmul_nt
-from ..ops.norms import _LayerNormFn
+from ..ops.norms import _LayerNormFn, colearn_add_layer_norm
 from .base import ColearnModel
-from .bert import BertConfig
+from .bert import BertConfig, MaskedAttentionMixin, document_ids
 from .stacked import SLinear
 
 
@@ -50,6 +51,15 @@ class SLayerNorm(nn.Module):
         y, _, _ = _LayerNormFn.apply(x, self.weight, self.bias, self.eps,
                                      self.G, self.gslot_w, self.gslot_b)
         return y
+
+    def add(self, x: torch.Tensor, branch: torch.Tensor) -> torch.Tensor:
+        """The norm of ``x + branch``, in one kernel."""
+        direct = (self.gslot_w is not None and x.is_cuda
+                  and native_enabled())
+        return colearn_add_layer_norm(
+            branch, x, self.weight, self.bias, self.eps, self.G,
+            self.gslot_w if direct else None,
+            self.gslot_b if direct else None)[0]
 
 
 class SEmbedding(nn.Module):
@@ -71,26 +81,30 @@ class SEmbedding(nn.Module):
         return out.reshape(*ids.shape, self.weight.shape[-1])
 
 
-class SBertSelfAttention(nn.Module):
+class SBertSelfAttention(nn.Module, MaskedAttentionMixin):
     def __init__(self, G: int, cfg: BertConfig) -> None:
         super().__init__()
+        self._init_masked(cfg)
         self.h = cfg.num_heads
         self.dh = cfg.hidden_size // cfg.num_heads
         self.qkv = SLinear(G, cfg.hidden_size, 3 * cfg.hidden_size)
         self.out = SLinear(G, cfg.hidden_size, cfg.hidden_size)
-        self.drop = nn.Dropout(cfg.dropout)
+        self.drop = nn.Dropout(cfg.probs_dropout)
         # fused-attention dropout stream: deterministic run-to-run
         # (keyed on the module's creation-time torch seed + call count)
         self._seed_base = int(torch.initial_seed()) & 0x7FFFFFFF
         self._call = 0
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, doc=None) -> torch.Tensor:
         from ..ops.attention import (
             fused_attention, fused_attention_applicable,
         )
 
         b, s, d = x.shape  # b = G*B
         qkv = self.qkv(x.reshape(b * s, d)).view(b, s, 3, self.h, self.dh)
+        if self.masked:
+            ctx = self._masked_attention(qkv, doc)
+            return self.out(ctx.reshape(b * s, d)).view(b, s, d)
         if fused_attention_applicable(qkv):
             p = float(self.drop.p) if self.training else 0.0
             self._call += 1
@@ -120,13 +134,17 @@ class SBertLayer(nn.Module):
         self.fc2 = SLinear(G, cfg.intermediate_size, cfg.hidden_size)
         self.ln2 = SLayerNorm(G, cfg.hidden_size, cfg.layer_norm_eps)
         self.drop = nn.Dropout(cfg.dropout)
+        self.fused_add_norm = cfg.fused_add_norm
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _join(self, ln: SLayerNorm, x: torch.Tensor,
+              branch: torch.Tensor) -> torch.Tensor:
+        return ln.add(x, branch) if self.fused_add_norm else ln(x + branch)
+
+    def forward(self, x: torch.Tensor, doc=None) -> torch.Tensor:
         b, s, d = x.shape
-        x = self.ln1(x + self.drop(self.attn(x)))
+        x = self._join(self.ln1, x, self.drop(self.attn(x, doc)))
         ff = self.fc2(colearn_gelu(self.fc1(x.reshape(b * s, d)))).view(b, s, d)
-        x = self.ln2(x + self.drop(ff))
-        return x
+        return self._join(self.ln2, x, self.drop(ff))
 
 
 class StackedBert(ColearnModel):
@@ -157,8 +175,9 @@ class StackedBert(ColearnModel):
         if torch.is_autocast_enabled("cuda") and x.is_cuda:
             x = x.to(torch.get_autocast_dtype("cuda"))
         x = self.drop(self.emb_ln(x))
+        doc = document_ids(ids, self.cfg)
         for layer in self.layers:
-            x = layer(x)
+            x = layer(x, doc)
         return x
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:

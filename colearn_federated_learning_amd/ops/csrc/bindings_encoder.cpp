@@ -520,9 +520,13 @@ struct AddNormFn : public torch::autograd::Function<AddNormFn> {
                                OptTensor gslot_w, OptTensor gslot_b) {
     auto [y, s, mean, inv] =
         add_norm_fwd(x, residual, weight, bias, eps, groups);
-    ctx->save_for_backward({s, weight, mean, inv,
-                            gslot_w.value_or(torch::Tensor()),
-                            gslot_b.value_or(torch::Tensor())});
+    ctx->save_for_backward({s, weight, mean, inv});
+    // Not saved as operands: they are written here, and they are views of a
+    // buffer that every other gradient is added into meanwhile.
+    if (gslot_w.has_value()) {
+      ctx->saved_data["gslot_w"] = *gslot_w;
+      ctx->saved_data["gslot_b"] = *gslot_b;
+    }
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["bias"] = bias.sizes().vec();
@@ -540,9 +544,10 @@ struct AddNormFn : public torch::autograd::Function<AddNormFn> {
       gx = grads[1];
     } else {
       const auto& weight = saved[1];
-      const bool direct = saved[4].defined();
-      auto gw = direct ? saved[4] : torch::empty_like(weight);
-      auto gb = direct ? saved[5]
+      const bool direct = ctx->saved_data.count("gslot_w") > 0;
+      auto gw = direct ? ctx->saved_data["gslot_w"].toTensor()
+                       : torch::empty_like(weight);
+      auto gb = direct ? ctx->saved_data["gslot_b"].toTensor()
                        : torch::empty(ctx->saved_data["bias"].toIntVector(),
                                       weight.options());
       OptTensor gs;
