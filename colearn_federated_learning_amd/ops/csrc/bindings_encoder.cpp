@@ -391,21 +391,23 @@ MaskedAttn describe(const torch::Tensor& q, const torch::Tensor& k,
   return a;
 }
 
-// (o [N, S, H, D], row statistics, summary of doc: empty if there is none)
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> masked_attn_fwd(
-    torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale,
-    bool causal, double softcap, OptTensor prefix, OptTensor doc,
-    OptTensor slopes) {
+// (o [N, S, H, D], what rounding took from it: empty if no backward pass
+// follows; row statistics, summary of doc: empty if there is none)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>
+masked_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                double scale, bool causal, double softcap, OptTensor prefix,
+                OptTensor doc, OptTensor slopes, bool train) {
   MaskedAttn a =
       describe(q, k, v, scale, causal, softcap, prefix, doc, slopes);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   auto o = torch::empty({a.N, a.S, a.H, a.D}, q.options());
+  auto rest = torch::empty({train ? o.numel() : 0}, q.options());
   auto lse = torch::empty({a.N, a.H, a.S}, q.options().dtype(torch::kFloat32));
   const int64_t tiles = (a.S + kAttnGroup - 1) / kAttnGroup;
   const bool summary = doc.has_value() && a.S > kAttnShort;
   auto sum = torch::empty({summary ? a.N * tiles : 0, 4},
                           q.options().dtype(torch::kInt32));
-  if (o.numel() == 0) return {o, lse, sum};
+  if (o.numel() == 0) return {o, rest, lse, sum};
   q = readable(q);
   k = readable(k);
   v = readable(v);
@@ -414,28 +416,33 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> masked_attn_fwd(
   a.v = view_of(v);
   a.o = view_of(o);
   a.lse = lse.data_ptr<float>();
+  if (train) a.rest = rest.data_ptr();
   if (summary) {
     a.tiles = reinterpret_cast<int4*>(sum.data_ptr<int>());
     launch_masked_attn_tiles(a, stream());
   }
   launch_masked_attn_fwd(a, elem_of(q, "q"), stream());
   HIP_CHECK_LAST();
-  return {o, lse, sum};
+  return {o, rest, lse, sum};
 }
 
 // Writes gq, gk, gv: any layout whose rows are contiguous and whose strides
 // and start are multiples of 8 elements.
 void masked_attn_bwd(torch::Tensor go, torch::Tensor q, torch::Tensor k,
-                     torch::Tensor v, torch::Tensor o, torch::Tensor lse,
-                     torch::Tensor sum, torch::Tensor gq, torch::Tensor gk,
-                     torch::Tensor gv, double scale, bool causal,
-                     double softcap, OptTensor prefix, OptTensor doc,
-                     OptTensor slopes) {
+                     torch::Tensor v, torch::Tensor o, torch::Tensor rest,
+                     torch::Tensor lse, torch::Tensor sum, torch::Tensor gq,
+                     torch::Tensor gk, torch::Tensor gv, double scale,
+                     bool causal, double softcap, OptTensor prefix,
+                     OptTensor doc, OptTensor slopes) {
   MaskedAttn a =
       describe(q, k, v, scale, causal, softcap, prefix, doc, slopes);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   check_like(go, q, "masked_attn: the output's gradient");
   check_like(o, q, "masked_attn: the output");
+  check_gpu(rest, q.device(), "masked_attn: the output's rest");
+  TORCH_CHECK(rest.scalar_type() == q.scalar_type() && rest.is_contiguous() &&
+                  rest.numel() == q.numel() && aligned16(rest),
+              "masked_attn: the output's rest does not match");
   check_like(gq, q, "masked_attn: q's gradient");
   check_like(gk, k, "masked_attn: k's gradient");
   check_like(gv, v, "masked_attn: v's gradient");
@@ -474,6 +481,7 @@ void masked_attn_bwd(torch::Tensor go, torch::Tensor q, torch::Tensor k,
   a.gq = view_of(gq);
   a.gk = view_of(gk);
   a.gv = view_of(gv);
+  a.rest = rest.data_ptr();
   a.lse = lse.data_ptr<float>();
   a.delta = delta.data_ptr<float>();
   if (sum.numel() > 0) a.tiles = reinterpret_cast<int4*>(sum.data_ptr<int>());
@@ -593,28 +601,29 @@ void run_masked_bwd(AutogradContext* ctx, const torch::Tensor& go,
   auto opt = [&](size_t i) -> OptTensor {
     return saved[i].defined() ? OptTensor(saved[i]) : OptTensor();
   };
-  masked_attn_bwd(go, q, k, v, saved[at], saved[at + 1], saved[at + 2], gq, gk,
-                  gv, ctx->saved_data["scale"].toDouble(),
+  masked_attn_bwd(go, q, k, v, saved[at], saved[at + 1], saved[at + 2],
+                  saved[at + 3], gq, gk, gv,
+                  ctx->saved_data["scale"].toDouble(),
                   ctx->saved_data["causal"].toBool(),
-                  ctx->saved_data["softcap"].toDouble(), opt(at + 3),
-                  opt(at + 4), opt(at + 5));
+                  ctx->saved_data["softcap"].toDouble(), opt(at + 4),
+                  opt(at + 5), opt(at + 6));
 }
 
 struct MaskedAttnFn : public torch::autograd::Function<MaskedAttnFn> {
   static torch::Tensor forward(AutogradContext* ctx, torch::Tensor q,
                                torch::Tensor k, torch::Tensor v, double scale,
                                bool causal, double softcap, OptTensor prefix,
-                               OptTensor doc, OptTensor slopes) {
-    auto [o, lse, sum] = masked_attn_fwd(q, k, v, scale, causal, softcap,
-                                         prefix, doc, slopes);
-    keep_masks(ctx, scale, causal, softcap, {q, k, v, o, lse, sum}, prefix,
-               doc, slopes);
+                               OptTensor doc, OptTensor slopes, bool train) {
+    auto [o, rest, lse, sum] = masked_attn_fwd(
+        q, k, v, scale, causal, softcap, prefix, doc, slopes, train);
+    keep_masks(ctx, scale, causal, softcap, {q, k, v, o, rest, lse, sum},
+               prefix, doc, slopes);
     return o;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    variable_list out(9);
+    variable_list out(10);
     for (int i = 0; i < 3; ++i)
       out[i] = torch::empty(saved[i].sizes(), saved[i].options());
     run_masked_bwd(ctx, grads[0], saved[0], saved[1], saved[2], saved, 3,
@@ -629,19 +638,19 @@ struct MaskedAttnQKVFn : public torch::autograd::Function<MaskedAttnQKVFn> {
   static torch::Tensor forward(AutogradContext* ctx, torch::Tensor qkv,
                                double scale, bool causal, double softcap,
                                OptTensor prefix, OptTensor doc,
-                               OptTensor slopes) {
-    auto [o, lse, sum] =
-        masked_attn_fwd(qkv.select(2, 0), qkv.select(2, 1), qkv.select(2, 2),
-                        scale, causal, softcap, prefix, doc, slopes);
-    keep_masks(ctx, scale, causal, softcap, {qkv, o, lse, sum}, prefix, doc,
-               slopes);
+                               OptTensor slopes, bool train) {
+    auto [o, rest, lse, sum] = masked_attn_fwd(
+        qkv.select(2, 0), qkv.select(2, 1), qkv.select(2, 2), scale, causal,
+        softcap, prefix, doc, slopes, train);
+    keep_masks(ctx, scale, causal, softcap, {qkv, o, rest, lse, sum}, prefix,
+               doc, slopes);
     return o;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const auto& qkv = saved[0];
-    variable_list out(7);
+    variable_list out(8);
     auto g = torch::empty(qkv.sizes(), qkv.options());
     run_masked_bwd(ctx, grads[0], qkv.select(2, 0), qkv.select(2, 1),
                    qkv.select(2, 2), saved, 1, g.select(2, 0), g.select(2, 1),
@@ -672,8 +681,11 @@ torch::Tensor masked_attention(torch::Tensor q, torch::Tensor k,
                                double softcap, OptTensor prefix, OptTensor doc,
                                OptTensor slopes) {
   const Masks m(prefix, doc, slopes);
+  const bool train = at::GradMode::is_enabled() &&
+                     (q.requires_grad() || k.requires_grad() ||
+                      v.requires_grad());
   return MaskedAttnFn::apply(q, k, v, scale, causal, softcap, m.prefix, m.doc,
-                             m.slopes);
+                             m.slopes, train);
 }
 
 // [N, S, H * D]
@@ -682,8 +694,9 @@ torch::Tensor masked_attention_qkv(torch::Tensor qkv, double scale,
                                    OptTensor prefix, OptTensor doc,
                                    OptTensor slopes) {
   const Masks m(prefix, doc, slopes);
+  const bool train = at::GradMode::is_enabled() && qkv.requires_grad();
   return MaskedAttnQKVFn::apply(qkv, scale, causal, softcap, m.prefix, m.doc,
-                                m.slopes)
+                                m.slopes, train)
       .flatten(2);
 }
 

@@ -94,6 +94,9 @@ struct HeadView {  // [N, S, heads, D] with D contiguous
 struct MaskedAttn {
   HeadView q, k, v, o;        // o: [N, S, H, D]
   HeadView go, gq, gk, gv;    // backward only
+  // What rounding took from o, in o's type and [N, S, H, D]; null if no
+  // backward pass follows.
+  void* rest;
   const int* doc;             // [N, S], or null
   const int* prefix;          // [N], or null
   const float* slopes;        // [H], or null
@@ -112,6 +115,9 @@ struct MaskedAttn {
 // 12 heads of size 64, us with two waves / with one: forward 1 x 4096 tokens
 // (384 workgroups) 79 / 94, 2 x 4096 (768) 161 / 136; dq 98 / 117 and
 // 198 / 172; dk/dv 1 x 2048 (192) 46 / 56, 1 x 4096 (384) 155 / 141.
+// The forward and dq also do for sequences of up to 64 tokens, where half of a
+// workgroup's 128 would be past the end: 2048 x 32 forward 228 / 250.  dk/dv
+// does not: 369 / 337.
 bool masked_attn_split(const MaskedAttn& a, int heads, int per_cu);
 // into how many shares dk/dv divides the heads of a key head
 int masked_attn_shares(const MaskedAttn& a);

@@ -35,33 +35,69 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
   const int there = min(own, a.S - 1);
   own_rows<DP>(row_of(a.q, n, h) + there * a.q.ss, a.D, qf);
   own_rows<DP>(row_of(a.go, n, h) + there * a.go.ss, a.D, gf);
+  const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S + own;
   float delta = 0.f, lse = INFINITY;
   {
-    const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S + own;
-    s16x8 of[DP / 16];
+    s16x8 of[DP / 16], rf[DP / 16];
     own_rows<DP>(row_of(a.o, n, h) + there * a.o.ss, a.D, of);
+    own_rows<DP>(static_cast<const short*>(a.rest) +
+                     ((static_cast<int64_t>(n) * a.S + there) * a.H + h) * a.D,
+                 a.D, rf);
     clear<DP>(live, a.D, qf);
     clear<DP>(live, a.D, gf);
     clear<DP>(live, a.D, of);
+    clear<DP>(live, a.D, rf);
     typedef __attribute__((ext_vector_type(8))) typename Bits16<T>::hw V;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
       const V g = __builtin_bit_cast(V, gf[kk]);
       const V o = __builtin_bit_cast(V, of[kk]);
+      const V r = __builtin_bit_cast(V, rf[kk]);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        delta += static_cast<float>(g[j]) * static_cast<float>(o[j]);
+        delta += static_cast<float>(g[j]) *
+                 (static_cast<float>(o[j]) + static_cast<float>(r[j]));
     }
     delta += other_half(delta);
-    if (own < a.S) {
-      lse = a.lse[stat];
-      if (half == 0 && part == 0) a.delta[stat] = delta;
-    }
+    if (own < a.S) lse = a.lse[stat];
   }
   const Score<M> sc(a, h);
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
+  Lift<T> lift;
+
+  // probabilities z, 2^up times as large, and dp - delta, of half kb of a tile;
+  // w: what the cap takes from dz
+  auto scores = [&](int buf, int kb, int t0, bool mixed, float up, f32x16& z,
+                    f32x16& dp, f32x16& w) {
+    const char* kt = sm.tile[buf][0] + kb * (L::kBytes / 2);
+    const char* vt = sm.tile[buf][1] + kb * (L::kBytes / 2);
+    const int other = kb * 32 + 4 * half;
+    z = 0.f;
+    dp = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      z = mfma<T>(L::rows(kt, kk), qf[kk], z);
+      dp = mfma<T>(L::rows(vt, kk), gf[kk], dp);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] -= delta;
+    if constexpr (M == kCap) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float th = fast_tanh(z[r] * sc.cap_in);
+        w[r] = 1.f - th * th;
+      }
+    }
+    const float lane_part =
+        sc.c * sc.shape(z, static_cast<float>(own - t0 - other),
+                        own_wave - t0 - kb * 32) - lse + up;
+    if (mixed) mask<true>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, lane_part));
+  };
 
   settle(qf);
   settle(gf);
@@ -95,6 +131,22 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
     keep(0, entry);
     arrived();
     __syncthreads();
+    if (KS == 2 && tiles <= kList && count == 1) {
+      // all that the rows attend to is here: D from p and dp themselves (in
+      // the variant of short sequences; in the other it would cost registers)
+      float miss = 0.f;
+      const int t0 = first_of(entry, base);
+      const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
+      for (int kb = 0; kb < 2; ++kb) {
+        const unsigned c = (cls >> (2 * kb)) & 3;
+        if (c == 0) continue;
+        f32x16 z, dp, w;
+        scores(0, kb, t0, c == 1, 0.f, z, dp, w);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) miss = __builtin_fmaf(z[r], dp[r], miss);
+      }
+      delta += miss + other_half(miss);
+    }
     for (int e = 0; e < count; ++e) {
       const int buf = e & 1;
       if (e + 1 < count) fetch(buf ^ 1, next);
@@ -106,32 +158,15 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
         const int kb = KS == 1 ? i : part;
         const unsigned c = (cls >> (2 * kb)) & 3;
         if (c == 0) continue;
+        f32x16 z, dp, w;
+        scores(buf, kb, t0, c == 1, lift.log2(), z, dp, w);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          dp[r] *= z[r];
+          if constexpr (M == kCap) dp[r] *= w[r];
+        }
+        lift.fit(dp, acc);
         const char* kt = sm.tile[buf][0] + kb * (L::kBytes / 2);
-        const char* vt = sm.tile[buf][1] + kb * (L::kBytes / 2);
-        const int other = kb * 32 + 4 * half;
-        f32x16 z = 0.f, dp = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          z = mfma<T>(L::rows(kt, kk), qf[kk], z);
-          dp = mfma<T>(L::rows(vt, kk), gf[kk], dp);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] -= delta;
-        if constexpr (M == kCap) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float th = fast_tanh(z[r] * sc.cap_in);
-            dp[r] *= 1.f - th * th;
-          }
-        }
-        const float lane_part =
-            sc.c * sc.shape(z, static_cast<float>(own - t0 - other),
-                            own_wave - t0 - kb * 32);
-        if (c == 1)
-          mask<true>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          dp[r] *= fast_exp2(__builtin_fmaf(z[r], sc.c, lane_part - lse));
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const s16x8 x = round8<T>(dp, s);
@@ -147,6 +182,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
       __syncthreads();
     }
   }
+  lift.leave(acc);
   // of the tile buffers: this wave's own part, or its pair's
   char* const mine =
       &sm.tile[0][0][0] +
@@ -162,6 +198,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) acc[i] += o[i];
   }
+  if (own < a.S && half == 0) a.delta[stat] = delta;
   store_cols<T, DP>(mine,
                     static_cast<T*>(a.gq.p) + n * a.gq.sn + h * a.gq.sh,
                     a.gq.ss, own_wave, a.S, acc, a.scale, live, a.D);
@@ -196,6 +233,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = 0.f;
+  Lift<T> lift;
 
   // half qb of the streamed tile; mixed: some pairs of it are not attended
   auto work = [&](const Score<M>& sc, int buf, int qb, int t0, bool mixed) {
@@ -224,6 +262,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
         dp[r] *= 1.f - th * th;
       }
     }
+    const float up = fast_exp2(lift.log2() - kLift<T>);
     sc.shape(z, static_cast<float>(own - t0 - other));
     if (mixed)
       mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
@@ -235,11 +274,11 @@ masked_attn_dkv_kernel(MaskedAttn a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = g * 4 + j;
-        z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -l4[j]));
-        dp[r] *= z[r];
-        z[r] *= kLift<T>;
+        z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -l4[j]));  // 2^kLift p
+        dp[r] *= z[r] * up;
       }
     }
+    lift.fit(dp, dk);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const s16x8 p = round8<T>(z, s);
@@ -289,7 +328,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
         if (threadIdx.x < kTile) {
           const bool past = t0 + static_cast<int>(threadIdx.x) >= a.S;
           sm.doc[buf][threadIdx.x] = docs.own(t0, a.S);
-          sm.lse[buf][threadIdx.x] = past ? INFINITY : lr;
+          sm.lse[buf][threadIdx.x] = past ? INFINITY : lr - kLift<T>;
           sm.delta[buf][threadIdx.x] = past ? 0.f : er;
         }
       };
@@ -297,7 +336,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       unsigned next = entry_of(sm.list, 1, count);
       fetch(0, entry);
       keep(0, entry);
-          arrived();
+      arrived();
       __syncthreads();
       for (int e = 0; e < count; ++e) {
         const int buf = e & 1;
@@ -319,6 +358,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       }
     }
   }
+  lift.leave(dk);
   char* const mine = &sm.tile[0][0][0] +
                      (KS == 2 ? (wave / 2) * DP * kWave * 4 : wave * DP * kWave);
   if constexpr (KS == 2) {
@@ -344,7 +384,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
     float* at = a.partial + share * size +
                 ((static_cast<int64_t>(n) * a.S + own) * a.Hkv + hk) * a.D;
     put_cols<DP>(at, dk, a.scale, live, a.D);
-    put_cols<DP>(at + a.shares * size, dv, 1.f / kLift<T>, live, a.D);
+    put_cols<DP>(at + a.shares * size, dv, fast_exp2(-kLift<T>), live, a.D);
     return;
   }
   store_cols<T, DP>(mine,
@@ -352,7 +392,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
                     a.gk.ss, own_wave, a.S, dk, a.scale, live, a.D);
   store_cols<T, DP>(mine,
                     static_cast<T*>(a.gv.p) + n * a.gv.sn + hk * a.gv.sh,
-                    a.gv.ss, own_wave, a.S, dv, 1.f / kLift<T>, live, a.D);
+                    a.gv.ss, own_wave, a.S, dv, fast_exp2(-kLift<T>), live, a.D);
 }
 
 // Shares' sums, four elements a thread: grid.y 0 dk, 1 dv.
@@ -387,7 +427,7 @@ struct Backward {
 
   template <typename T, int DP, Mode M>
   void run() const {
-    if (masked_attn_split(a, a.H, 2))
+    if (a.S <= kTile || masked_attn_split(a, a.H, 2))
       masked_attn_dq_kernel<T, DP, M, 2>
           <<<a.N * a.H * ((a.S + 63) / 64), 256, 0, stream>>>(a);
     else

@@ -204,9 +204,23 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
   }
   // NaN in a live row's sum is kept: only an empty row is cleared
   const bool empty = !live || l == 0.f;
+  const float f = empty ? 0.f : 1.f / l;
   store_cols<T, DP>(mine,
                     static_cast<T*>(a.o.p) + n * a.o.sn + h * a.o.sh, a.o.ss,
-                    own_wave, a.S, acc, empty ? 0.f : 1.f / l, !empty, a.D);
+                    own_wave, a.S, acc, f, !empty, a.D);
+  if (a.rest != nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = acc[i][r] * f;
+        acc[i][r] = x - elem_round(x, static_cast<const T*>(nullptr));
+      }
+    const int64_t row = static_cast<int64_t>(a.H) * a.D;
+    store_cols<T, DP>(mine,
+                      static_cast<T*>(a.rest) + n * a.S * row + h * a.D, row,
+                      own_wave, a.S, acc, 1.f, !empty, a.D);
+  }
   if (own < a.S && half == 0)
     a.lse[(static_cast<int64_t>(n) * a.H + h) * a.S + own] =
         empty ? INFINITY : m + log2f(l);
@@ -219,7 +233,7 @@ struct Forward {
   template <typename T, int DP, Mode M>
   void run() const {
     const int heads = a.N * a.H;
-    if (masked_attn_split(a, a.H, 2))
+    if (a.S <= kTile || masked_attn_split(a, a.H, 2))
       masked_attn_fwd_kernel<T, DP, M, 2>
           <<<heads * ((a.S + 63) / 64), 256, 0, stream>>>(a);
     else

@@ -11,9 +11,11 @@ Statistics and sums are fp32: a probability is off by the score's error, a few
 steps of 2^-24 times the score's size and the length of its sum, covered by
 f = 2^-17 (1 + max|z|) relative.
 float16 rounds what lies below 2^-14 to multiples of 2^-24, off by e = 2^-25
-whatever its size: e on every dz, and in the forward e on every probability
-relative to its row's largest (e max(p_i) on p_ij).  The backward's p is
-rounded 2^15 times as large, so that e 2^-15 is left of it.
+whatever its size: in the forward e on every probability relative to its row's
+largest (e max(p_i) on p_ij).  The backward's p is rounded 2^15 times as large,
+so that e 2^-15 is left of it; and dz times a power of two with which the
+largest of its query (for dq), or of its key and the heads that share it (for
+dk), is 2^5 at least, which leaves e 2^-5 of that largest.
 """
 
 import math
@@ -40,6 +42,7 @@ def _oracle(q, k, v, go, scale, causal=False, prefix=None, doc=None,
     dk, dv = torch.zeros_like(k), torch.zeros_like(k)
     to, tq = torch.zeros_like(q), torch.zeros_like(q)
     tk, tv = torch.zeros_like(k), torch.zeros_like(k)
+    top, near = torch.zeros(n, k.shape[2], s).double(), torch.zeros_like(k)
     pos = torch.arange(s)
     for b in range(n):
         live = torch.ones(s, dtype=torch.bool)
@@ -83,11 +86,14 @@ def _oracle(q, k, v, go, scale, causal=False, prefix=None, doc=None,
             bigerr = (g.abs() * (2 * u + rel) * (ob.abs() + pv)).sum(
                 1, keepdim=True)
             ez = u * dz.abs() + p * f * (bigerr + rel * (dpa + big.abs()))
-            ez = ez + e * ok
+            low = e * 2.0 ** -5 * ok.double()
             dq[b, :, a] = dz @ y * scale
-            tq[b, :, a] = ez @ y.abs() * scale
+            tq[b, :, a] = (ez + low * dz.abs().amax(1, True)) @ y.abs() * scale
             dk[b, :, c] += dz.T @ x * scale
+            top[b, c] = torch.maximum(top[b, c], dz.abs().amax(0))
             tk[b, :, c] += ez.T @ x.abs() * scale
+            near[b, :, c] += low.T @ x.abs() * scale
+    tk += near * top.transpose(1, 2)[..., None]
     tq += u * dq.abs() + 1e-9
     tk += u * dk.abs() + 1e-9
     tv += u * dv.abs() + 1e-9
@@ -204,6 +210,31 @@ def test_softcap(dev, cap):
 def test_distance(dev, h):
     _check(dev, 1, 300, h, h, 64, torch.bfloat16, packed=True,
            slopes=distance_slopes(h), doc=_docs(1, 300, 2, 120))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("s,cap", [(40, 0.0), (700, 0.0), (700, 20.0)])
+@pytest.mark.parametrize("small", [2.0 ** -14, 2.0 ** -10, 2.0 ** 10])
+def test_small_and_large_gradients_in_float16(dev, s, cap, small):
+    """dz below and above what float16 holds.  q and k are large where the
+    other's gradient is looked at, so that it is not itself too small, or too
+    large, for the type."""
+    g = torch.Generator().manual_seed(s)
+    big = 2.0 ** (-4 if small > 1 else 6)
+    for name in ("dq", "dk"):
+        q, k, v, go = (torch.randn(2, s, 2, 32, generator=g)
+                       for _ in range(4))
+        q, k = (q / big, k * big) if name == "dq" else (q * big, k / big)
+        go[:, ::3] *= 2.0 ** -6  # some rows' far smaller than others'
+        q, k, v, go = (t.to(torch.float16).to(dev).requires_grad_()
+                       for t in (q, k, v, go * small))
+        out = colearn_attention(q, k, v, softcap=cap)
+        i = 0 if name == "dq" else 1
+        got = torch.autograd.grad(out, (q, k), go)[i].cpu().double()
+        want, tol = _oracle(q, k, v, go, 32 ** -0.5, softcap=cap)
+        assert torch.isfinite(got).all()
+        worst = ((got - want[1 + i]).abs() / tol[1 + i]).max().item()
+        assert worst <= 1.0, f"{name}: {worst:.2f} times its tolerance"
 
 
 @pytest.mark.parametrize("dev", DEVICES)
