@@ -15,7 +15,6 @@ layout-independent, and regenerated in the backward (csrc/attn.hip).
 
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
@@ -114,10 +113,11 @@ def _check_masked(q, k, v, scale, causal, softcap, prefix, doc, slopes):
     if not (q.dtype == k.dtype == v.dtype) or not q.is_floating_point():
         raise TypeError(f"q, k and v must have one floating type, got "
                         f"{q.dtype}, {k.dtype}, {v.dtype}")
-    if not scale > 0.0:
-        raise ValueError(f"the scale must be positive, got {scale}")
-    if not 0.0 <= softcap < math.inf:
-        raise ValueError(f"softcap must be finite and not negative, got "
+    if not 1e-18 <= scale <= 1e18:
+        raise ValueError(f"the scale must be within 1e-18 and 1e18, got "
+                         f"{scale}")
+    if softcap != 0.0 and not 1e-18 <= softcap <= 1e18:
+        raise ValueError(f"softcap must be 0 or within 1e-18 and 1e18, got "
                          f"{softcap}")
     if prefix is not None:
         if not causal:
@@ -155,8 +155,9 @@ def colearn_attention(
     """Self-attention of q [N, S, H, D] over k, v [N, S, Hkv, D]; returns
     [N, S, H, D].  Key head ``h // (H // Hkv)`` serves head ``h``.
 
-    - ``scale``: of the scores, positive (default ``D ** -0.5``)
-    - ``softcap``: scores become ``softcap * tanh(score / softcap)`` (0: not)
+    - ``scale``: of the scores, 1e-18 to 1e18 (default ``D ** -0.5``)
+    - ``softcap``: scores become ``softcap * tanh(score / softcap)`` (0: not;
+      else within the same bounds)
     - ``slopes`` float32 [H]: ``slopes[h] * |i - j|`` is taken off the score
       of query i and key j (after the cap); constants, without gradient
     - ``causal``: a query attends to keys up to its own position; with
@@ -164,7 +165,9 @@ def colearn_attention(
     - ``doc`` int32 [N, S]: a query attends to keys of its own document only;
       negative marks padding, whose outputs and gradients are zeros and whose
       values (NaN and infinities included) reach no other token.  Ids need not
-      be sorted; packed rows (each document in one piece) cost least.
+      be sorted; packed rows (each document in one piece) cost least.  A NaN or
+      an infinity in a token that is not padding may reach every token of its
+      sequence, masked or not (0 times it is NaN).
 
     Gradients of q, k and v are bitwise the same from run to run.  bfloat16 and
     float16 operands on the GPU with D a multiple of 8 up to 128 run the HIP

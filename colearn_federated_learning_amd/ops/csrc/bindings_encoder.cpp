@@ -28,6 +28,10 @@ namespace colearn {
 
 namespace {
 
+// a launch has fewer than 2^32 threads
+constexpr int64_t kMostThreads = std::numeric_limits<uint32_t>::max();
+constexpr int64_t kMostBlocks = kMostThreads / 256;  // of 256 threads
+
 using OptTensor = std::optional<torch::Tensor>;
 
 hipStream_t stream() {
@@ -91,7 +95,7 @@ void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
   TORCH_CHECK(real(pt) && real(gt),
               "adamw: parameters and gradients must be float32 or bfloat16");
   const auto state = eight ? torch::kFloat8_e4m3fn : torch::kFloat32;
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
   written.reserve(count * (eight ? 5 : 3));
   auto check = [&](const torch::Tensor& t, torch::ScalarType type, int64_t n,
                    bool out, const char* name) {
@@ -101,9 +105,9 @@ void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
                 ", not ", t.scalar_type());
     TORCH_CHECK(t.is_contiguous() && t.numel() == n, "adamw: ", name,
                 " must be contiguous with ", n, " elements");
-    if (out && n > 0) {
+    if (n > 0) {
       const auto a = reinterpret_cast<uintptr_t>(t.data_ptr());
-      written.emplace_back(a, a + t.nbytes());
+      (out ? written : read).emplace_back(a, a + t.nbytes());
     }
   };
   for (size_t i = 0; i < count; ++i) {
@@ -124,6 +128,14 @@ void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
     TORCH_CHECK(written[i - 1].second <= written[i].first,
                 "adamw: a tensor that the step writes is there twice, or two "
                 "of them overlap");
+  for (const auto& [first, last] : read) {
+    const auto next = std::lower_bound(
+        written.begin(), written.end(), first,
+        [](const auto& w, uintptr_t x) { return w.second <= x; });
+    TORCH_CHECK(next == written.end() || last <= next->first,
+                "adamw: a gradient or reference overlaps a tensor that the "
+                "step writes");
+  }
   AdamwScalars sc{};
   sc.b1 = static_cast<float>(b1);
   sc.omb1 = static_cast<float>(1.0 - b1);
@@ -157,11 +169,11 @@ void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
     const int64_t n = p[i].numel();
     if (n == 0) continue;
     const int64_t groups = (n + kAdamwChunk - 1) / kAdamwChunk;
-    TORCH_CHECK(groups < std::numeric_limits<int>::max(),
-                "adamw: a tensor of ", n, " elements is too long");
-    if (tab.count == kAdamwTensors ||
-        grid + groups > std::numeric_limits<int>::max())
-      flush();
+    TORCH_CHECK(groups <= kMostBlocks, "adamw: a tensor of ", n,
+                " elements is too long");
+    if (tab.count == kAdamwTensors || grid + groups > kMostBlocks) flush();
+    // whoever saved the parameter for a backward pass has to learn of this
+    if (!p[i].is_inference()) p[i].unsafeGetTensorImpl()->bump_version();
     AdamwTensor& t = tab.t[tab.count];
     t.p = p[i].data_ptr();
     t.g = g[i].data_ptr();
@@ -199,8 +211,9 @@ void check_norm(const torch::Tensor& x, const torch::Tensor& w,
   TORCH_CHECK(groups >= 1 && groups <= 65535 && *rows % groups == 0,
               "add_norm: ", *rows, " rows do not divide into ", groups,
               " groups");
-  TORCH_CHECK(*rows < std::numeric_limits<int>::max(),
-              "add_norm: too many rows");
+  const int64_t threads = *H <= 1024 ? 64 : *H <= 4096 ? 256 : 1024;  // a row
+  TORCH_CHECK(*rows <= kMostThreads / threads - 3, "add_norm: too many rows (",
+              *rows, ")");
   check_gpu(w, x.device(), "add_norm: weight");
   TORCH_CHECK(w.scalar_type() == torch::kFloat32 && w.is_contiguous() &&
                   w.numel() == groups * *H,
@@ -346,13 +359,17 @@ MaskedAttn describe(const torch::Tensor& q, const torch::Tensor& k,
                     D);
   constexpr int64_t kMost = std::numeric_limits<int>::max();
   TORCH_CHECK_VALUE(
-      S <= (1 << 22) && N <= kMost && N * H * ((S + 63) / 64) <= kMost,
-      "attention: too many tokens (a sequence has at most 2^22)");
-  TORCH_CHECK_VALUE(scale > 0.0 && scale <= std::numeric_limits<float>::max(),
-                    "attention: the scale must be positive, got ", scale);
+      S <= (1 << 22) && N <= kMost && H <= kMost && N * H <= kMost &&
+          N * H * ((S + 63) / 64) <= kMostBlocks,
+      "attention: too many tokens (a sequence has at most 2^22, all heads of "
+      "all sequences 2^24 tiles of 64)");
+  // the kernels form scale / softcap and slope / scale in fp32
+  TORCH_CHECK_VALUE(scale >= 1e-18 && scale <= 1e18,
+                    "attention: the scale must be within 1e-18 and 1e18, got ",
+                    scale);
   TORCH_CHECK_VALUE(
-      softcap >= 0.0 && softcap <= std::numeric_limits<float>::max(),
-      "attention: softcap must be finite and not negative, got ", softcap);
+      softcap == 0.0 || (softcap >= 1e-18 && softcap <= 1e18),
+      "attention: softcap must be 0 or within 1e-18 and 1e18, got ", softcap);
   MaskedAttn a{};
   a.N = static_cast<int>(N);
   a.S = static_cast<int>(S);
@@ -550,6 +567,10 @@ struct AddNormFn : public torch::autograd::Function<AddNormFn> {
     torch::Tensor gx;
     if (!grads[0].defined()) {  // only the sum was used
       gx = grads[1];
+      if (ctx->saved_data.count("gslot_w") > 0) {
+        ctx->saved_data["gslot_w"].toTensor().zero_();
+        ctx->saved_data["gslot_b"].toTensor().zero_();
+      }
     } else {
       const auto& weight = saved[1];
       const bool direct = ctx->saved_data.count("gslot_w") > 0;
@@ -577,6 +598,14 @@ std::tuple<torch::Tensor, torch::Tensor> add_layer_norm(
     torch::Tensor x, OptTensor residual, torch::Tensor weight,
     torch::Tensor bias, double eps, int64_t groups, OptTensor gslot_w,
     OptTensor gslot_b) {
+  for (const auto& g : {gslot_w, gslot_b}) {
+    if (!g.has_value()) continue;
+    check_gpu(*g, x.device(), "add_norm: a gradient slot");
+    TORCH_CHECK(g->scalar_type() == torch::kFloat32 && g->is_contiguous() &&
+                    g->numel() == weight.numel(),
+                "add_norm: gradient slots must be contiguous float32 of "
+                "weight's size");
+  }
   auto out = AddNormFn::apply(x, residual, weight, bias, eps, groups, gslot_w,
                               gslot_b);
   return {out[0], out[1]};

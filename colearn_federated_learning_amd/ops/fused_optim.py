@@ -262,7 +262,7 @@ def adamw_step(
 
     Parameters are all float32 or all bfloat16 (rounded to nearest), and so
     are gradients; everything is contiguous and on one device, and no tensor
-    that is written may overlap another.  ``live``: float32 ``[lr / bc1,
+    that is written may overlap another operand.  ``live``: float32 ``[lr / bc1,
     1 / bc2]`` on the device, read by the kernel in place of what ``step`` and
     ``lr`` give (a captured graph's arguments are frozen).
     """

@@ -311,7 +311,8 @@ def colearn_add_layer_norm(
     (overwriting them) and returns none, as the stacked engine's norms do.
 
     float32, bfloat16 and float16 on the GPU, rows up to 16384, run the HIP
-    kernels (csrc/add_norm.hip); the parameters are float32.  Other operands
+    kernels (csrc/add_norm.hip; up to 2^26 rows of 1024, 2^24 of 4096, 2^22 of
+    more elements); the parameters are float32.  Other operands
     run the same formulas in torch (without gslots).  A residual of another
     type is joined in the wider of the two.
     """

@@ -307,6 +307,38 @@ def test_captured_and_replayed(bits):
                 assert torch.equal(_codes(a), _codes(b))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_saved_parameter_is_missed(dev):
+    p = torch.ones(40, device=dev, requires_grad=True)
+    loss = (p * p).sum()
+    m, v, _, _ = adamw_state([p], 32)
+    adamw_step([p], [torch.ones(40, device=dev)], m, v, step=1, lr=0.1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+
+
+@pytest.mark.gpu
+def test_more_than_32_bits_of_elements():
+    n, tail = 2 ** 31 + 300, 2 ** 31 - 512
+    g = torch.Generator("cuda").manual_seed(0)
+    p, grad = (torch.empty(n, dtype=torch.bfloat16, device="cuda")
+               .normal_(generator=g) for _ in range(2))
+    states = adamw_state([p], 8)
+    few = [p[tail:].clone()]
+    few_states = adamw_state(few, 8)
+    for k in (1, 2):
+        for ps, gs, (m, v, ms, vs) in (
+                ([p], [grad], states), (few, [grad[tail:].clone()],
+                                        few_states)):
+            adamw_step(ps, gs, m, v, exp_avg_scales=ms, exp_avg_sq_scales=vs,
+                       step=k, lr=0.1)
+    assert torch.equal(p[tail:], few[0])
+    for a, b in zip(states[:2], few_states[:2]):
+        assert torch.equal(_codes(a[0][tail:]), _codes(b[0]))
+    for a, b in zip(states[2:], few_states[2:]):
+        assert torch.equal(a[0][tail // 256:], b[0])
+
+
 @pytest.mark.gpu
 def test_another_stream():
     a, b = _steps("cuda", 8), None
@@ -355,6 +387,10 @@ def test_refusals(dev):
                exp_avg_sq_scales=vs)
         refuse(bad, [p[0], p[0]], g, m, v)  # the same tensor twice
         refuse(bad, p, g, m, m)
+        refuse(bad, p, [g[0], p[0]], m, v)  # read where it is written
+        refuse(bad, p, g, m, v, fedprox_mu=0.1, refs=[p[1], g[0]])
+        both = torch.zeros(301, device=dev)
+        refuse(bad, [both[1:], p[1]], [both[:300], g[1]], m, v)
         flat = torch.zeros(400, device=dev)
         refuse(bad, [flat[:300], flat[100:]], g, m, v)  # overlapping
         wide = torch.zeros(300, 2, device=dev)

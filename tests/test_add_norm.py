@@ -178,6 +178,45 @@ def test_same_norm_as_the_module(dev):
 
 
 @pytest.mark.gpu
+def test_slots_are_zeros_where_only_the_sum_is_used():
+    x, w = (torch.ones(6, 8, device="cuda", requires_grad=True)
+            for _ in range(2))
+    slots = [torch.full((6, 8), math.nan, device="cuda") for _ in range(2)]
+    _, s = colearn_add_layer_norm(x, x.detach(), w, w, groups=6,
+                                  gslot_w=slots[0], gslot_b=slots[1])
+    s.sum().backward()
+    assert (x.grad == 1).all() and all((t == 0).all() for t in slots)
+
+
+@pytest.mark.gpu
+def test_more_than_32_bits_of_elements():
+    rows, h = 2 ** 21 + 5, 1024
+    g = torch.Generator("cuda").manual_seed(0)
+    x = torch.empty(rows, h, dtype=torch.bfloat16, device="cuda")
+    x.normal_(generator=g)
+    gy = torch.zeros_like(x)
+    ends = torch.cat([torch.arange(8), torch.arange(rows - 8, rows)]).cuda()
+    gy[ends] = torch.randn(16, h, generator=g, device="cuda").to(x.dtype)
+    w, b = (torch.randn(h, generator=g, device="cuda").requires_grad_()
+            for _ in range(2))
+
+    def run(x, gy):
+        x = x.requires_grad_()
+        y, s = colearn_add_layer_norm(x, x.detach(), w, b)
+        return [y, s, *torch.autograd.grad(y, (x, w, b), gy)]
+
+    few = run(x[ends], gy[ends])
+    all_ = run(x, gy)
+    for a, c in zip(all_[:3], few[:3]):
+        assert torch.equal(a[ends], c)
+    # sums of the same 16 terms in another order: 15 roundings each, of 2^-24
+    # of what the terms add up to; a normalised element is at most 32
+    most = gy[ends].float().abs().sum(0) * 32
+    for a, c in zip(all_[3:], few[3:]):
+        assert ((a - c).abs() <= 2 * 15 * 2.0 ** -24 * most).all()
+
+
+@pytest.mark.gpu
 def test_slots_order_streams_and_replay():
     g = torch.Generator().manual_seed(0)
     x, r, gy = (torch.randn(64, 96, generator=g).to(torch.bfloat16).cuda()
@@ -277,6 +316,10 @@ def test_refusals(dev):
     refuse(TypeError, x.int(), None, w, w)
     refuse(ValueError, x, None, w, w, gslot_w=w)
     if dev == "cuda":
+        for bad in (w[:7], w.half(), w.cpu(), torch.ones(16, device=dev)[::2]):
+            refuse(RuntimeError, x, None, w, w, gslot_w=w.clone(), gslot_b=bad)
+        many = torch.zeros(2 ** 26, 1, dtype=torch.bfloat16, device=dev)
+        refuse(RuntimeError, many, None, w[:1], w[:1])
         refuse(ValueError, x, None, w.cpu(), w)
         refuse(TypeError, x, None, w.half(), w.half())
         y, _ = colearn_add_layer_norm(x.requires_grad_(), None, w, w)

@@ -455,6 +455,9 @@ def test_refusals(dev):
     refuse(TypeError, q.int(), kv.int(), kv.int())
     refuse(ValueError, q, kv, kv, scale=0.0)
     refuse(ValueError, q, kv, kv, scale=-1.0)
+    for x in (1e-30, 1e30, math.inf, math.nan):
+        refuse(ValueError, q, kv, kv, scale=x)
+        refuse(ValueError, q, kv, kv, softcap=x)
     refuse(ValueError, q, kv, kv, softcap=-1.0)
     refuse(ValueError, q, kv, kv, softcap=math.inf)
     refuse(ValueError, q, kv, kv, prefix=doc[:, 0])
@@ -485,3 +488,93 @@ def test_empty(dev):
         y = colearn_attention(x, x, x)
         y.sum().backward()
         assert y.shape == shape and x.grad.shape == shape
+    q = torch.zeros(2, 5, 0, 16, dtype=torch.bfloat16, device=dev)
+    k = torch.ones(2, 5, 2, 16, dtype=torch.bfloat16, device=dev,
+                   requires_grad=True)
+    y = colearn_attention(q.requires_grad_(), k, k)
+    y.sum().backward()
+    assert y.shape == q.shape and (k.grad == 0).all()
+
+
+def _check_part(part, x, out, gr, go, doc=None):
+    """Rows `part` of a fused projection x, whose documents lie within it."""
+    q, k, v = (t[:, part].detach().cpu() for t in x.unbind(2))
+    go = go[:, part].reshape(q.shape).cpu()
+    doc = None if doc is None else doc[:, part].cpu()
+    want, tol = _oracle(q, k, v, go, q.shape[-1] ** -0.5, doc=doc)
+    got = (out[:, part].reshape(q.shape), *gr[:, part].unbind(2))
+    for name, y, w, t in zip(("out", "dq", "dk", "dv"), got, want, tol):
+        worst = ((y.detach().cpu().double() - w).abs() / t).max().item()
+        assert worst <= 1.0, f"{name}: {worst:.2f} times its tolerance"
+
+
+@pytest.mark.gpu
+def test_sequences_more_than_32_bits_apart():
+    n = 130 * 3 * 2 * 64
+    far = torch.empty(2 ** 31 + n, dtype=torch.bfloat16, device="cuda")
+    x = far.as_strided((2, 130, 3, 2, 64), (2 ** 31, 384, 128, 64, 1))
+    g = torch.Generator().manual_seed(0)
+    near = torch.randn(2, 130, 3, 2, 64, generator=g).to(torch.bfloat16)
+    x.copy_(near)
+    go = torch.randn(2, 130, 128, generator=g).to(torch.bfloat16).cuda()
+    y = x.detach().requires_grad_()
+    out = colearn_attention_qkv(y)
+    (gr,) = torch.autograd.grad(out, y, go)
+    near = near.cuda().requires_grad_()
+    want = colearn_attention_qkv(near)
+    assert torch.equal(out, want)
+    assert torch.equal(gr, torch.autograd.grad(want, near, go)[0])
+
+
+@pytest.mark.gpu
+def test_more_than_32_bits_of_elements():
+    """One row of 2^20 tokens in documents of 128: o, and each gradient, have
+    2^31 elements."""
+    s, h, d = 2 ** 20, 16, 128
+    g = torch.Generator("cuda").manual_seed(0)
+    x = torch.empty(1, s, 3, h, d, dtype=torch.bfloat16, device="cuda")
+    x.normal_(generator=g).requires_grad_()
+    doc = (torch.arange(s, dtype=torch.int32, device="cuda") // 128)[None]
+    go = torch.empty(1, s, h * d, dtype=torch.bfloat16, device="cuda")
+    go.normal_(generator=g)
+    out = colearn_attention_qkv(x, doc=doc)
+    (gr,) = torch.autograd.grad(out, x, go)
+    for part in (slice(0, 256), slice(s // 2 - 128, s // 2 + 128),
+                 slice(s - 256, s)):
+        _check_part(part, x, out, gr, go, doc)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    g = torch.Generator().manual_seed(0)
+    xs = [torch.randn(2, 700, 3, 4, 64, generator=g).to(torch.bfloat16).cuda()
+          for _ in range(2)]
+    doc = _docs(2, 700, 1, 200).cuda()
+    go = torch.randn(2, 700, 256, generator=g).to(torch.bfloat16).cuda()
+
+    def run(x):
+        y = x.clone().requires_grad_()
+        out = colearn_attention_qkv(y, doc=doc)
+        return out.detach(), torch.autograd.grad(out, y, go)[0]
+
+    want = [run(x) for x in xs]
+    sides = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(run(xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(a, want[i]))
+
+
+@pytest.mark.gpu
+def test_functional_gradient():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(1, 70, 3, 2, 64, generator=g).to(torch.bfloat16).cuda()
+    go = torch.randn(1, 70, 128, generator=g).to(torch.bfloat16).cuda()
+    out, pull = torch.func.vjp(colearn_attention_qkv, x)
+    _check_part(slice(0, 70), x, out, pull(go)[0], go)
