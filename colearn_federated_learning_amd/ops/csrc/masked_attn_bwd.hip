@@ -209,6 +209,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void
 masked_attn_dkv_kernel(MaskedAttn a) {
   using L = Tile<DP>;
   constexpr int OWN = 128 / KS, KB = 2 / KS;
+  // Both halves of a tile at once where there is a distance to work out: 1 x
+  // 4096 tokens, 12 heads of size 64, 174 us, one after the other 185.
+  // Not without (short documents: 78 and 75), nor with the cap (no registers).
+  constexpr bool kJoint = KS == 1 && DP <= 64 && M == kBias;
   __shared__ __align__(16) Smem<DP> sm;
   int n, hs, own0;  // hs: key head and share
   locate<OWN>(a, a.Hkv * a.shares, false, &n, &hs, &own0);
@@ -235,58 +239,72 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = 0.f;
   Lift<T> lift;
 
-  // half qb of the streamed tile; mixed: some pairs of it are not attended
-  auto work = [&](const Score<M>& sc, int buf, int qb, int t0, bool mixed) {
-    const char* qt = sm.tile[buf][0] + qb * (L::kBytes / 2);
-    const char* gt = sm.tile[buf][1] + qb * (L::kBytes / 2);
-    const int other = qb * 32 + 4 * half;
-    f32x16 z = 0.f, dp = 0.f;
+  // N halves of the streamed tile from half qb on; cls: their marks
+  auto work = [&](auto number, const Score<M>& sc, int buf, int qb, int t0,
+                  unsigned cls) {
+    constexpr int N = decltype(number)::value;
+    f32x16 zs[N], dps[N];
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      z = mfma<T>(L::rows(qt, kk), kf[kk], z);
-      dp = mfma<T>(L::rows(gt, kk), vf[kk], dp);
-    }
+    for (int i = 0; i < N; ++i) {
+      const char* qt = sm.tile[buf][0] + (qb + i) * (L::kBytes / 2);
+      const char* gt = sm.tile[buf][1] + (qb + i) * (L::kBytes / 2);
+      zs[i] = 0.f;
+      dps[i] = 0.f;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float4 de =
-          *reinterpret_cast<const float4*>(sm.delta[buf] + other + g * 8);
-      dp[g * 4] -= de.x;
-      dp[g * 4 + 1] -= de.y;
-      dp[g * 4 + 2] -= de.z;
-      dp[g * 4 + 3] -= de.w;
-    }
-    if constexpr (M == kCap) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float th = fast_tanh(z[r] * sc.cap_in);
-        dp[r] *= 1.f - th * th;
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        zs[i] = mfma<T>(L::rows(qt, kk), kf[kk], zs[i]);
+        dps[i] = mfma<T>(L::rows(gt, kk), vf[kk], dps[i]);
       }
     }
-    const float up = fast_exp2(lift.log2() - kLift<T>);
-    sc.shape(z, static_cast<float>(own - t0 - other));
-    if (mixed)
-      mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float4 ls =
-          *reinterpret_cast<const float4*>(sm.lse[buf] + other + g * 8);
-      const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
+    for (int i = 0; i < N; ++i) {
+      const char* qt = sm.tile[buf][0] + (qb + i) * (L::kBytes / 2);
+      const char* gt = sm.tile[buf][1] + (qb + i) * (L::kBytes / 2);
+      const int other = (qb + i) * 32 + 4 * half;
+      f32x16& z = zs[i];
+      f32x16& dp = dps[i];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = g * 4 + j;
-        z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -l4[j]));  // 2^kLift p
-        dp[r] *= z[r] * up;
+      for (int g = 0; g < 4; ++g) {
+        const float4 de =
+            *reinterpret_cast<const float4*>(sm.delta[buf] + other + g * 8);
+        dp[g * 4] -= de.x;
+        dp[g * 4 + 1] -= de.y;
+        dp[g * 4 + 2] -= de.z;
+        dp[g * 4 + 3] -= de.w;
       }
-    }
-    lift.fit(dp, dk);
+      if constexpr (M == kCap) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const s16x8 p = round8<T>(z, s);
-      const s16x8 x = round8<T>(dp, s);
+        for (int r = 0; r < 16; ++r) {
+          const float th = fast_tanh(z[r] * sc.cap_in);
+          dp[r] *= 1.f - th * th;
+        }
+      }
+      const float up = fast_exp2(lift.log2() - kLift<T>);
+      sc.shape(z, static_cast<float>(own - t0 - other));
+      if (((cls >> (2 * i)) & 3) != 2)
+        mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) {
-        dv[db] = mfma<T>(L::cols(gt, s, db), p, dv[db]);
-        dk[db] = mfma<T>(L::cols(qt, s, db), x, dk[db]);
+      for (int g = 0; g < 4; ++g) {
+        const float4 ls =
+            *reinterpret_cast<const float4*>(sm.lse[buf] + other + g * 8);
+        const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = g * 4 + j;
+          z[r] = fast_exp2(__builtin_fmaf(z[r], sc.c, -l4[j]));  // 2^kLift p
+          dp[r] *= z[r] * up;
+        }
+      }
+      lift.fit(dp, dk);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const s16x8 p = round8<T>(z, s);
+        const s16x8 x = round8<T>(dp, s);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+          dv[db] = mfma<T>(L::cols(gt, s, db), p, dv[db]);
+          dk[db] = mfma<T>(L::cols(qt, s, db), x, dk[db]);
+        }
       }
     }
   };
@@ -344,11 +362,17 @@ masked_attn_dkv_kernel(MaskedAttn a) {
         const unsigned after = sm.list[min(e + 2, count - 1)];
         const int t0 = first_of(entry, base);
         const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
+        if constexpr (kJoint) {
+          if (cls != 0)
+            work(std::integral_constant<int, 2>(), sc, buf, 0, t0, cls);
+        } else {
 #pragma unroll
-        for (int i = 0; i < KB; ++i) {
-          const int qb = KS == 1 ? i : part;
-          const unsigned c = (cls >> (2 * qb)) & 3;
-          if (c != 0) work(sc, buf, qb, t0, c == 1);
+          for (int i = 0; i < KB; ++i) {
+            const int qb = KS == 1 ? i : part;
+            const unsigned c = (cls >> (2 * qb)) & 3;
+            if (c != 0)
+              work(std::integral_constant<int, 1>(), sc, buf, qb, t0, c);
+          }
         }
         if (e + 1 < count) keep(buf ^ 1, next);
         entry = next;
