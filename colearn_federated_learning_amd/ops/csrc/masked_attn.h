@@ -15,11 +15,11 @@
 // double-buffered: the next tile's loads are issued before a tile is worked
 // on and land in the other buffer after it.  A workgroup's four waves own 128
 // tokens (KS = 1), or 64 with two waves on each 32, one for either half of
-// every tile, joined through LDS at the end (KS = 2).  Products are 32x32x16 MFMAs with
-// the streamed side as the left operand, so that a lane's column of the
-// result belongs to one owned token and its 16 registers to streamed tokens:
-// the softmax is a reduction over registers plus one exchange between the
-// wave's halves, and the rounded probabilities already lie as the right
+// every tile, joined through LDS at the end (KS = 2; KS = 8: eight waves own
+// 128 like that).  Products are 32x32x16 MFMAs with the streamed side as the
+// left operand, so that a lane's column of the result belongs to one owned
+// token and its 16 registers to streamed tokens: the softmax is a reduction
+// over registers plus one exchange between the wave's halves, and the rounded probabilities already lie as the right
 // operand of the second product.  That operand's k order is
 //     slot 8h + j  <->  token 4h + (j & 3) + 8 (j >> 2)       (h: lane / 32)
 // instead of the plain one; the left operand, read transposed from the same
@@ -179,8 +179,6 @@ DEV_INLINE float other_half(float x) { return swap32(x); }
 template <int DP>
 struct Tile {
   static constexpr int kSlots = DP / 8;
-  static constexpr int kStep = 256 / kSlots;       // rows a pass of all threads
-  static constexpr int kPer = kTile / kStep;       // passes
   static constexpr int kBytes = kTile * DP * 2;
 
   DEV_INLINE static int at(int row, int slot) {
@@ -213,12 +211,14 @@ struct Tile {
   }
 };
 
-// One streamed operand [S, D] on its way into LDS.  Each of a tile's kPer
-// passes moves 16 bytes a thread.  A row's offset in a tile is 32 bits of
+// One streamed operand [S, D] on its way into LDS, by W waves.  Each of a tile's
+// kPer passes moves 16 bytes a thread.  A row's offset in a tile is 32 bits of
 // bytes (the host sees to it), the tile's own 64.
-template <int DP>
+template <int DP, int W = 4>
 struct Stream {
   using L = Tile<DP>;
+  static constexpr int kStep = W * kWave / L::kSlots;  // rows a pass
+  static constexpr int kPer = kTile / kStep;           // passes
   const short* base;
   int64_t ss;
 
@@ -243,13 +243,13 @@ struct Stream {
         static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)lds)) +
         wave * 1024);
 #pragma unroll
-    for (int i = 0; i < L::kPer; ++i)
+    for (int i = 0; i < kPer; ++i)
       asm volatile(
           "s_mov_b32 m0, %0\n\t"
           "s_nop 0\n\t"
           "global_load_lds_dwordx4 %1, %2"
           :
-          : "s"(to + i * 4096), "v"(off), "s"(p + i * L::kStep * step)
+          : "s"(to + i * (W * 1024)), "v"(off), "s"(p + i * kStep * step)
           : "memory", "m0");
   }
   // Any tile: rows that `live` has no bit of, and columns past D, as zeros.
@@ -259,8 +259,8 @@ struct Stream {
     const unsigned step = static_cast<unsigned>(2 * ss);
     const char* p = reinterpret_cast<const char*>(base + t0 * ss);
 #pragma unroll
-    for (int i = 0; i < L::kPer; ++i) {
-      const int row = row0 + i * L::kStep;
+    for (int i = 0; i < kPer; ++i) {
+      const int row = row0 + i * kStep;
       s16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
       if (slot * 8 < D && ((live >> row) & 1))
         x = *reinterpret_cast<const s16x8*>(p + row * step + slot * 16);
@@ -416,7 +416,7 @@ DEV_INLINE const int4* summary_of(const MaskedAttn& a, int n, int4* lds) {
   const int groups = (a.S + 31) / 32;
   if (a.tiles != nullptr) return a.tiles + static_cast<int64_t>(n) * groups;
   const int* doc = a.doc + static_cast<int64_t>(n) * a.S;
-  for (int t0 = 0; t0 < a.S; t0 += 256) {
+  for (int t0 = 0; t0 < a.S; t0 += static_cast<int>(blockDim.x)) {
     const int t = t0 + threadIdx.x;
     const int4 s = summarise(doc[min(t, a.S - 1)], t < a.S);
     if (threadIdx.x % 32 == 0 && t < a.S) lds[t / 32] = s;
@@ -604,9 +604,10 @@ DEV_INLINE int pair_limit(const MaskedAttn& a, int n, int own) {
   return own < prefix ? 0 : own;
 }
 
-template <int DP>
+template <int DP, bool OWN = false>
 struct Smem {
   char tile[2][2][Tile<DP>::kBytes];  // buffer, operand
+  char own[OWN ? 2 : 0][2][Tile<DP>::kBytes];  // operand, 64 tokens
   int doc[2][kTile];
   float lse[2][kTile];    // dk/dv only
   float delta[2][kTile];  // dk/dv only

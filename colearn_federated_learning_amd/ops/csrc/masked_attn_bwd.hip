@@ -204,16 +204,28 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
                     a.gq.ss, own_wave, a.S, acc, a.scale, live, a.D);
 }
 
+// Both sums of 32 keys of size 128 take 128 registers and the keys' own rows
+// another 64: one wave a SIMD, with nothing to run while it waits.  KS = 8 is
+// for those: two waves a SIMD, eight to a workgroup, in pairs like KS = 2, with
+// the own rows in LDS.  Less to run beside a workgroup's begin and end, so for
+// long sequences: 8 x 2048 tokens, 16 heads, 678 us, KS = 1 775; 16 x 1024 437
+// and 456; 32 x 512, 12 heads, 196 and 184.
+constexpr int kEight = 1024;
+
 template <typename T, int DP, Mode M, int KS>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void
+__global__ __launch_bounds__(KS == 8 ? 512 : 256,
+                             DP == 128 && KS != 8 ? 1 : 2) void
 masked_attn_dkv_kernel(MaskedAttn a) {
   using L = Tile<DP>;
-  constexpr int OWN = 128 / KS, KB = 2 / KS;
+  constexpr bool kLds = KS == 8;
+  constexpr int W = kLds ? 8 : 4;
+  constexpr int PAIR = kLds ? 2 : KS;  // waves that share 32 owned tokens
+  constexpr int OWN = 32 * W / PAIR, KB = 2 / PAIR;
   // Both halves of a tile at once where there is a distance to work out: 1 x
   // 4096 tokens, 12 heads of size 64, 174 us, one after the other 185.
   // Not without (short documents: 78 and 75), nor with the cap (no registers).
   constexpr bool kJoint = KS == 1 && DP <= 64 && M == kBias;
-  __shared__ __align__(16) Smem<DP> sm;
+  __shared__ __align__(16) Smem<DP, kLds> sm;
   int n, hs, own0;  // hs: key head and share
   locate<OWN>(a, a.Hkv * a.shares, false, &n, &hs, &own0);
   const int hk = hs / a.shares, share = hs % a.shares;
@@ -221,8 +233,8 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   const int group = a.H / a.Hkv / a.shares;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
-  const int half = lane >> 5, part = KS == 1 ? 0 : wave & 1;
-  const int own_wave = own0 + (wave / KS) * 32;
+  const int half = lane >> 5, part = PAIR == 1 ? 0 : wave & 1;
+  const int own_wave = own0 + (wave / PAIR) * 32;
   const int own = own_wave + (lane & 31);
   const int found = doc_of(a, n, own);
   const bool live = found >= 0;
@@ -230,10 +242,24 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   const int lim = pair_limit<false>(a, n, own);
   Docs docs(a, n);
   const int4* sum = summary_of(a, n, sm.sum);
-  s16x8 kf[DP / 16], vf[DP / 16];
-  const int there = min(own, a.S - 1);
-  own_rows<DP>(row_of(a.k, n, hk) + there * a.k.ss, a.D, kf);
-  own_rows<DP>(row_of(a.v, n, hk) + there * a.v.ss, a.D, vf);
+  s16x8 kf[kLds ? 1 : DP / 16], vf[kLds ? 1 : DP / 16];
+  const char *kt = nullptr, *vt = nullptr;  // this wave's rows in LDS
+  if constexpr (kLds) {
+    const Stream<DP, W> ks(row_of(a.k, n, hk), a.k.ss);
+    const Stream<DP, W> vs(row_of(a.v, n, hk), a.v.ss);
+    for (int i = 0; i < OWN / kTile; ++i) {
+      docs.load(own0 + i * kTile, a.S);
+      const unsigned long long there = docs.live(own0 + i * kTile, a.S);
+      ks.copy(sm.own[0][i], own0 + i * kTile, a.S, a.D, there);
+      vs.copy(sm.own[1][i], own0 + i * kTile, a.S, a.D, there);
+    }
+    kt = sm.own[0][0] + (wave / PAIR) * (L::kBytes / 2);
+    vt = sm.own[1][0] + (wave / PAIR) * (L::kBytes / 2);
+  } else {
+    const int there = min(own, a.S - 1);
+    own_rows<DP>(row_of(a.k, n, hk) + there * a.k.ss, a.D, kf);
+    own_rows<DP>(row_of(a.v, n, hk) + there * a.v.ss, a.D, vf);
+  }
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = 0.f;
@@ -252,8 +278,10 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       dps[i] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
-        zs[i] = mfma<T>(L::rows(qt, kk), kf[kk], zs[i]);
-        dps[i] = mfma<T>(L::rows(gt, kk), vf[kk], dps[i]);
+        zs[i] = mfma<T>(L::rows(qt, kk), kLds ? L::rows(kt, kk) : kf[kk],
+                        zs[i]);
+        dps[i] = mfma<T>(L::rows(gt, kk), kLds ? L::rows(vt, kk) : vf[kk],
+                         dps[i]);
       }
     }
 #pragma unroll
@@ -308,10 +336,12 @@ masked_attn_dkv_kernel(MaskedAttn a) {
       }
     }
   };
-  clear<DP>(live, a.D, kf);
-  clear<DP>(live, a.D, vf);
-  settle(kf);
-  settle(vf);
+  if constexpr (!kLds) {
+    clear<DP>(live, a.D, kf);
+    clear<DP>(live, a.D, vf);
+    settle(kf);
+    settle(vf);
+  }
   const int tiles = (a.S + kTile - 1) / kTile;
   for (int base = 0; base < tiles; base += kList) {
     const int count = list_tiles<false, OWN / 32>(a, n, own0, base, sum,
@@ -320,8 +350,8 @@ masked_attn_dkv_kernel(MaskedAttn a) {
     for (int hi = 0; hi < group && count > 0; ++hi) {
       const int h = hs * group + hi;
       const Score<M> sc(a, h);
-      const Stream<DP> qs(row_of(a.q, n, h), a.q.ss);
-      const Stream<DP> gs(row_of(a.go, n, h), a.go.ss);
+      const Stream<DP, W> qs(row_of(a.q, n, h), a.q.ss);
+      const Stream<DP, W> gs(row_of(a.go, n, h), a.go.ss);
       const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S;
       float lr, er;
       auto fetch = [&](int buf, unsigned entry) {
@@ -361,14 +391,14 @@ masked_attn_dkv_kernel(MaskedAttn a) {
         if (e + 1 < count) fetch(buf ^ 1, next);
         const unsigned after = sm.list[min(e + 2, count - 1)];
         const int t0 = first_of(entry, base);
-        const unsigned cls = (entry >> (4 * (wave / KS))) & 15;
+        const unsigned cls = (entry >> (4 * (wave / PAIR))) & 15;
         if constexpr (kJoint) {
           if (cls != 0)
             work(std::integral_constant<int, 2>(), sc, buf, 0, t0, cls);
         } else {
 #pragma unroll
           for (int i = 0; i < KB; ++i) {
-            const int qb = KS == 1 ? i : part;
+            const int qb = PAIR == 1 ? i : part;
             const unsigned c = (cls >> (2 * qb)) & 3;
             if (c != 0)
               work(std::integral_constant<int, 1>(), sc, buf, qb, t0, c);
@@ -383,9 +413,11 @@ masked_attn_dkv_kernel(MaskedAttn a) {
     }
   }
   lift.leave(dk);
+  // of the tile buffers (KS = 8: and the own rows behind them)
   char* const mine = &sm.tile[0][0][0] +
-                     (KS == 2 ? (wave / 2) * DP * kWave * 4 : wave * DP * kWave);
-  if constexpr (KS == 2) {
+                     (PAIR == 2 ? (wave / 2) * DP * kWave * 4
+                                : wave * DP * kWave);
+  if constexpr (PAIR == 2) {
     float* at = reinterpret_cast<float*>(mine);
     __syncthreads();
     if (part == 1) {
@@ -458,12 +490,15 @@ struct Backward {
       masked_attn_dq_kernel<T, DP, M, 1>
           <<<a.N * a.H * ((a.S + 127) / 128), 256, 0, stream>>>(a);
     const int heads = a.Hkv * a.shares;
+    const int blocks = a.N * heads * ((a.S + 127) / 128);
     if (masked_attn_split(a, heads, 1))
       masked_attn_dkv_kernel<T, DP, M, 2>
           <<<a.N * heads * ((a.S + 63) / 64), 256, 0, stream>>>(a);
+    else if (DP == 128 && a.S >= kEight)
+      masked_attn_dkv_kernel<T, DP, M, DP == 128 ? 8 : 1>
+          <<<blocks, 512, 0, stream>>>(a);
     else
-      masked_attn_dkv_kernel<T, DP, M, 1>
-          <<<a.N * heads * ((a.S + 127) / 128), 256, 0, stream>>>(a);
+      masked_attn_dkv_kernel<T, DP, M, 1><<<blocks, 256, 0, stream>>>(a);
     if (a.shares > 1) {
       const int64_t size = static_cast<int64_t>(a.N) * a.S * a.Hkv * a.D;
       masked_attn_join_kernel<T>
@@ -478,8 +513,8 @@ struct Backward {
 int masked_attn_shares(const MaskedAttn& a) {
   // Key heads that serve several heads leave the dk/dv grid short: the group
   // is shared out until there are two workgroups a CU, or every head has its
-  // own.  2 x 1999 capped tokens, 16 heads over 4, size 128:
-  // 281 us in one share, 227 + 13 (the join) in four.
+  // own.  2 x 1999 capped tokens, 16 heads over 4, size 128: with the join, 281
+  // us in one share, 255 in two, 246 in four.
   const int group = a.H / a.Hkv;
   const int64_t blocks =
       static_cast<int64_t>(a.N) * a.Hkv * ((a.S + 127) / 128);

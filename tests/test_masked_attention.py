@@ -237,6 +237,39 @@ def test_small_and_large_gradients_in_float16(dev, s, cap, small):
         assert worst <= 1.0, f"{name}: {worst:.2f} times its tolerance"
 
 
+MANY = {
+    "plain": {},
+    "causal": dict(causal=True),
+    "documents": dict(doc=_docs(20, 257, 5, 70)),
+    "distance": dict(slopes=distance_slopes(12), doc=_docs(20, 257, 6, 150)),
+    "cap": dict(softcap=8.0, causal=True,
+                prefix=torch.arange(0, 260, 13, dtype=torch.int32)),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", MANY)
+@pytest.mark.parametrize("d,dtype", [
+    (32, torch.float16), (64, torch.bfloat16), (64, torch.float16),
+    (128, torch.bfloat16)])
+def test_many_sequences(kind, d, dtype):
+    """Grids that fill the chip with a wave on every 32 tokens."""
+    _check("cuda", 20, 257, 12, 12, d, dtype, seed=d, packed=True,
+           **MANY[kind])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dtype,h,hkv,kw", [
+    (72, torch.bfloat16, 4, 4, dict(doc=_docs(8, 1090, 5, 300))),
+    (128, torch.bfloat16, 4, 4, dict(slopes=distance_slopes(4))),
+    (128, torch.float16, 8, 2, dict(softcap=8.0, causal=True,
+                                    doc=_docs(8, 1090, 7, 800))),
+    (128, torch.float16, 4, 4, {}),
+])
+def test_long_rows_of_large_heads(d, dtype, h, hkv, kw):
+    _check("cuda", 8, 1090, h, hkv, d, dtype, seed=d, **kw)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_everything_at_once(dev):
     doc = _docs(2, 530, 4, 200)
