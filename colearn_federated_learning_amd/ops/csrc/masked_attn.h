@@ -47,6 +47,13 @@
 // sum 23 of 290 for 512 x 64; in every tile it would be 4 of 176, for nothing
 // that shows.
 //
+// What bounds them: vector operations in the forward (a score costs an
+// exponential, at a quarter of the rate, and four more), registers in the
+// backward, where two to three waves a SIMD cover little of each other's
+// latency.  Without masks, forward / dq / dk/dv in TFLOP/s (4, 6 and 8 D
+// operations a pair): 32 x 512 tokens, 12 heads of 64, 540 / 630 / 675; 2 x
+// 8192 825 / 985 / 951; 8 x 2048, 16 heads of 128, 820 / 980 / 811.
+//
 // Scores are held in base 2 (scale * log2 e folded in) and every statistic in
 // fp32.  Probabilities and dz are rounded to the operands' type for the second
 // products; the sums in the denominator are of the unrounded ones.
