@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops import is_vmapped
 from ..ops.attention import colearn_attention_qkv, distance_slopes
 from ..ops.gemm import colearn_linear, colearn_matmul, colearn_matmul_nt
 from ..ops.norms import ColearnLayerNorm, colearn_add_layer_norm
@@ -108,9 +109,12 @@ class MaskedAttentionMixin:
         """[b, s, 3, h, dh] -> [b, s, h * dh]"""
         slopes = None
         if self.distance_bias:
-            if self._slopes is None or self._slopes.device != qkv.device:
-                self._slopes = distance_slopes(self.h, qkv.device)
             slopes = self._slopes
+            if slopes is None or slopes.device != qkv.device:
+                slopes = distance_slopes(self.h, qkv.device)
+                # not one that lives in a transform or is closed to autograd
+                if not (is_vmapped() or torch.is_inference_mode_enabled()):
+                    self._slopes = slopes
         return colearn_attention_qkv(qkv, doc=doc, softcap=self.softcap,
                                      slopes=slopes)
 

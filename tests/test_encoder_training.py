@@ -304,3 +304,36 @@ def test_example_runs():
         cwd=ROOT, capture_output=True, text=True, timeout=600)
     assert out.returncode == 0, out.stderr[-2000:]
     assert "round" in out.stdout
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("first", ["per_sample", "inference"])
+def test_training_after_a_transform_or_inference(dev, first):
+    """Per-sample gradients by functorch are those of each row alone, and
+    nothing that either leaves behind is in training's way."""
+    model = _bert(doc_sep_token=9, pad_token=0, attn_softcap=20.0,
+                  attn_distance_bias=True, fused_add_norm=True).to(dev)
+    ids = torch.randint(1, 64, (3, 60),
+                        generator=torch.Generator().manual_seed(3)).to(dev)
+    params = dict(model.named_parameters())
+
+    def loss(p, row):
+        return torch.func.functional_call(
+            model, p, (row[None],)).float().square().mean()
+
+    if first == "per_sample":
+        got = torch.func.vmap(torch.func.grad(loss), (None, 0))(
+            {k: p.detach() for k, p in params.items()}, ids)
+        for i in range(3):
+            want = torch.autograd.grad(loss(params, ids[i]),
+                                       list(params.values()))
+            for (k, g), w in zip(got.items(), want):
+                # float32 sums of another order, over tensors of 2^12 at most
+                assert ((g[i] - w).norm() <= 2.0 ** -14 * w.norm() + 1e-7), k
+    else:
+        with torch.inference_mode():
+            model(ids)
+    with torch.autocast("cuda", torch.bfloat16, enabled=dev == "cuda"):
+        out = model(ids).float().square().mean()
+    out.backward()
+    assert all(torch.isfinite(p.grad).all() for p in model.parameters())
