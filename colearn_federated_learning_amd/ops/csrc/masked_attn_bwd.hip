@@ -28,7 +28,6 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
   const int own_doc = live ? found : -2;
   const int lim = pair_limit<true>(a, n, own);
   Docs docs(a, n);
-  const int4* sum = summary_of(a, n, sm.sum);
   const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss);
   const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss);
   s16x8 qf[DP / 16], gf[DP / 16];
@@ -37,12 +36,14 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
   own_rows<DP>(row_of(a.go, n, h) + there * a.go.ss, a.D, gf);
   const int64_t stat = (static_cast<int64_t>(n) * a.H + h) * a.S + own;
   float delta = 0.f, lse = INFINITY;
+  const int4* sum;
   {
     s16x8 of[DP / 16], rf[DP / 16];
     own_rows<DP>(row_of(a.o, n, h) + there * a.o.ss, a.D, of);
     own_rows<DP>(static_cast<const short*>(a.rest) +
                      ((static_cast<int64_t>(n) * a.S + there) * a.H + h) * a.D,
                  a.D, rf);
+    sum = summary_of(a, n, sm.sum);
     clear<DP>(live, a.D, qf);
     clear<DP>(live, a.D, gf);
     clear<DP>(live, a.D, of);
@@ -241,7 +242,6 @@ masked_attn_dkv_kernel(MaskedAttn a) {
   const int own_doc = live ? found : -2;
   const int lim = pair_limit<false>(a, n, own);
   Docs docs(a, n);
-  const int4* sum = summary_of(a, n, sm.sum);
   s16x8 kf[kLds ? 1 : DP / 16], vf[kLds ? 1 : DP / 16];
   const char *kt = nullptr, *vt = nullptr;  // this wave's rows in LDS
   if constexpr (kLds) {
@@ -260,6 +260,7 @@ masked_attn_dkv_kernel(MaskedAttn a) {
     own_rows<DP>(row_of(a.k, n, hk) + there * a.k.ss, a.D, kf);
     own_rows<DP>(row_of(a.v, n, hk) + there * a.v.ss, a.D, vf);
   }
+  const int4* sum = summary_of(a, n, sm.sum);
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = 0.f;

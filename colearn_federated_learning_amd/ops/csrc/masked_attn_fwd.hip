@@ -45,11 +45,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
   const int own_doc = live ? found : -2;
   const int lim = pair_limit<true>(a, n, own);
   Docs docs(a, n);
+  s16x8 qf[DP / 16];
+  own_rows<DP>(row_of(a.q, n, h) + min(own, a.S - 1) * a.q.ss, a.D, qf);
   const int4* sum = summary_of(a, n, sm.sum);
   const Stream<DP> ks(row_of(a.k, n, hk), a.k.ss);
   const Stream<DP> vs(row_of(a.v, n, hk), a.v.ss);
-  s16x8 qf[DP / 16];
-  own_rows<DP>(row_of(a.q, n, h) + min(own, a.S - 1) * a.q.ss, a.D, qf);
   const Score<M> sc(a, h);
   f32x16 acc[DP / 32];
 #pragma unroll
