@@ -11,13 +11,14 @@
 // variance is the mean of squared distances from the mean: the row stays in
 // registers, so the second pass over it costs no memory.
 //
-// Bound by memory: 65536 x 768 in bf16, forward 73 us (5.5 TB/s), backward 62 and
-// the join 4 (4.6 TB/s); 4096 x 768, where a launch begins to show, 7 and 8 + 3;
-// 16384 x 1024 in fp32 56 and 33 + 4 (4.8, 5.4 TB/s).  A row's elements lie over W waves, at most 16 a lane
-// (W = 1 up to 1024 columns, 4 up to 4096, 16 up to 16384), so the backward
-// can hold both weight sums of its columns in registers over all its rows and
-// read everything once: each workgroup leaves one row of partial sums, which
-// a second launch adds up in a fixed order.
+// Bound by memory: 65536 x 768 in bf16, forward 74 us (5.4 TB/s), backward 58
+// to 62 and the join 4 (4.5 to 4.9 TB/s); 4096 x 768, where a launch begins to
+// show, 7 and 8 + 3; 16384 x 1024 in fp32 54 and 33 + 4 (5.0, 5.4 TB/s).  A
+// row's elements lie over W waves, at most 16 a lane (W = 1 up to 1024 columns,
+// 4 up to 4096, 16 up to 16384), so the backward can hold both weight sums of
+// its columns in registers over all its rows and read everything once: each
+// workgroup leaves one row of partial sums, which a second launch adds up in a
+// fixed order.
 
 #include "elem.h"
 #include "encoder_api.h"
@@ -182,34 +183,38 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void add_norm_bwd_kernel(
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kRows;
   int64_t q = static_cast<int64_t>(blockIdx.x) * kRows +
               (W == 1 ? threadIdx.x / kWave : 0);
-  // The next row's loads are under way while a row is reduced and written
-  // (not where 16 waves leave no registers for them).
-  constexpr bool kAhead = W < 16;
-  Raw<T, VEC> gr[NV], sr[NV];
-  float mu = 0.f, is = 0.f;
-  auto fetch = [&](int64_t row) {
-    mu = mean[row];
-    is = inv[row];
+  // The next rows' loads are under way while a row is reduced and written: two
+  // rows of 16-bit elements (65536 x 768 in 8 groups 58 us, one row 63; 8192 x
+  // 4096 37 and 41), one of 32-bit ones (4099 x 1023 21, two 24), none where 16
+  // waves leave no registers for them.
+  constexpr int kAhead = W == 16 ? 0 : sizeof(T) == 2 ? 2 : 1;
+  struct Row {
+    Raw<T, VEC> g[NV], s[NV];
+    float mu, is;
+  } rows[kAhead > 0 ? kAhead : 1];
+  auto fetch = [&](Row& to, int64_t row) {
+    to.mu = mean[row];
+    to.is = inv[row];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = min(col_of<VEC, W>(k), H - VEC);
-      gr[k] = load_raw<VEC>(gy + row * H + c);
-      sr[k] = load_raw<VEC>(s + row * H + c);
+      to.g[k] = load_raw<VEC>(gy + row * H + c);
+      to.s[k] = load_raw<VEC>(s + row * H + c);
     }
   };
-  if (kAhead && q < rpg) fetch(row0 + q);
-  for (; q < rpg; q += stride) {
+  auto work = [&](Row& in) {
     const int64_t row = row0 + q;
-    if (!kAhead) fetch(row);
+    if (kAhead == 0) fetch(in, row);
     float g[EL], xh[EL];
     float sum[2] = {0.f, 0.f};
-    const float m = mu, rs = is;
+    const float m = in.mu, rs = in.is;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      widen<VEC>(gr[k], g + k * VEC);
-      widen<VEC>(sr[k], xh + k * VEC);
+      widen<VEC>(in.g[k], g + k * VEC);
+      widen<VEC>(in.s[k], xh + k * VEC);
     }
-    if (kAhead && q + stride < rpg) fetch(row + stride);
+    if (kAhead > 0 && q + kAhead * stride < rpg)
+      fetch(in, row + kAhead * stride);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (col_of<VEC, W>(k) < H) {
@@ -247,6 +252,14 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void add_norm_bwd_kernel(
         store_vec<VEC>(gx + row * H + c, o);
       }
     }
+    q += stride;
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (q + i * stride < rpg) fetch(rows[i], row0 + q + i * stride);
+  while (q < rpg) {
+    work(rows[0]);
+    if (kAhead > 1 && q < rpg) work(rows[kAhead - 1]);
   }
   float* out = partials + (static_cast<int64_t>(blockIdx.y) * gridDim.x +
                            blockIdx.x) * 2 * H;
