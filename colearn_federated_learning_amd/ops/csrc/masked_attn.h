@@ -12,35 +12,36 @@
 // All three kernels have one shape.  A wave owns 32 tokens (queries in the
 // forward and dq kernels, keys in the dk/dv kernel) whose operands stay in
 // registers, and tiles of 64 tokens of the other side stream through LDS,
-// double-buffered: the next tile's loads are issued before a tile is worked
-// on and land in the other buffer after it.  A workgroup's four waves own 128
+// double-buffered: the next tile's loads are issued before a tile is worked on
+// and land in the other buffer after it.  A workgroup's four waves own 128
 // tokens (KS = 1), or 64 with two waves on each 32, one for either half of
 // every tile, joined through LDS at the end (KS = 2; KS = 8: eight waves own
 // 128 like that).  Products are 32x32x16 MFMAs with the streamed side as the
 // left operand, so that a lane's column of the result belongs to one owned
 // token and its 16 registers to streamed tokens: the softmax is a reduction
-// over registers plus one exchange between the wave's halves, and the rounded probabilities already lie as the right
-// operand of the second product.  That operand's k order is
+// over registers plus one exchange between the wave's halves, and the rounded
+// probabilities already lie as the right operand of the second product.  That
+// operand's k order is
 //     slot 8h + j  <->  token 4h + (j & 3) + 8 (j >> 2)       (h: lane / 32)
-// instead of the plain one; the left operand, read transposed from the same
-// LDS tile (ds_read_b64_tr_b16: four tokens of 16 columns a lane group), uses
-// the same order, so nothing moves between lanes.
+// instead of the plain one; the left operand, read transposed from the same LDS
+// tile (ds_read_b64_tr_b16: four tokens of 16 columns a lane group), uses the
+// same order, so nothing moves between lanes.
 //
 // In fp16 the backward rounds 2^15 p instead of p (the factor leaves dv again
-// in fp32): a uniform row of 16K tokens has p = 2^-14, below which fp16 loses
-// a bit for every halving.  dz is as small as the gradients are and has no
-// bound above: every owned token has a power of two for it that falls as its
-// largest dz so far asks for (`Lift`), and leaves its sum at the end.  11 x 3913
+// in fp32): a uniform row of 16K tokens has p = 2^-14, below which fp16 loses a
+// bit for every halving.  dz is as small as the gradients are and has no bound
+// above: every owned token has a power of two for it that falls as its largest
+// dz so far asks for (`Lift`), and leaves its sum at the end.  11 x 3913
 // tokens, go around 0.02: relative error of dq and dk 0.00030, and 0.00042
-// without.  2 x 1999 tokens, 16 heads of size 128: dq 137 us, 129 without, dk/dv
-// 232 and 227.
+// without.  2 x 1999 tokens, 16 heads of size 128: dq 137 us, 129 without,
+// dk/dv 232 and 227.
 //
 // dz is a small difference where few tokens share a row, and an error of D is
 // one of the whole row.  Taken from the rounded o it would be as large as dz's
 // own rounding, so the forward keeps what rounding took from o (in 16 bits).
 // That leaves the rounding of p in o, which matters where a handful of tokens
-// are all: sequences of up to 64 get D as the sum of p dp, in fp32, in a pass of
-// its own.  Relative error of dq, bf16: 6 causal tokens 0.0032 from the
+// are all: sequences of up to 64 get D as the sum of p dp, in fp32, in a pass
+// of its own.  Relative error of dq, bf16: 6 causal tokens 0.0032 from the
 // rounded o, 0.0025 with the rest, 0.0023 from the sum; documents of 150
 // 0.0026, 0.0024.  0.0017 is the rounding of the result alone.  The rest costs
 // 3 + 3 us of 176 where bytes count most (32 x 512 tokens, 12 heads, 64); the
@@ -62,9 +63,8 @@
 // padding).  A workgroup first lists the tiles that it has to visit, with a
 // mark for every 32 x 32 pairs: none attended (the wave skips them), all (no
 // test in the loop) or some; tiles between documents that do not meet cost
-// nothing.  Rows of padding are
-// staged as zeros and rows of padding are written as zeros, so that whatever
-// a padded token holds reaches no result.
+// nothing.  Rows of padding are staged as zeros and rows of padding are written
+// as zeros, so that whatever a padded token holds reaches no result.
 //
 // The backward recomputes p from the saved row statistic, in two kernels
 // without atomics (dq with D, then dk/dv): 7 products instead of the 5 of a
