@@ -33,8 +33,8 @@
 // above: every owned token has a power of two for it that falls as its largest
 // dz so far asks for (`Lift`), and leaves its sum at the end.  11 x 3913
 // tokens, go around 0.02: relative error of dq and dk 0.00030, and 0.00042
-// without.  2 x 1999 tokens, 16 heads of size 128: dq 137 us, 129 without,
-// dk/dv 232 and 227.
+// without.  2 x 1999 tokens, 16 heads of size 128: dq 137 us, 129 without;
+// dk/dv 2 % more.
 //
 // dz is a small difference where few tokens share a row, and an error of D is
 // one of the whole row.  Taken from the rounded o it would be as large as dz's
@@ -45,8 +45,9 @@
 // rounded o, 0.0025 with the rest, 0.0023 from the sum; documents of 150
 // 0.0026, 0.0024.  0.0017 is the rounding of the result alone.  The rest costs
 // 3 + 3 us of 176 where bytes count most (32 x 512 tokens, 12 heads, 64); the
-// sum 23 of 290 for 512 x 64; in every tile it would be 4 of 176, for nothing
-// that shows.
+// sum 23 of 290 for 512 x 64 (kept in registers over a barrier instead of
+// computed ahead: 9 more); in every tile it would be 4 of 176, for nothing that
+// shows.
 //
 // What bounds them: vector operations in the forward (a score costs an
 // exponential, at a quarter of the rate, and four more), registers in the
