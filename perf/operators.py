@@ -414,9 +414,7 @@ def _quantise(x, positive):
     blocks = F.pad(x, (0, -n % BLOCK)).view(-1, BLOCK)
     top = blocks.abs().amax(dim=1)
     live = top > TINY
-    # a division (a number over a tensor would be a rounded reciprocal's
-    # product): u may lie next to a border
-    inv = torch.where(live, torch.full_like(top, E4M3_MAX) / top, 0.0)
+    inv = torch.where(live, E4M3_MAX / top, 0.0)
     scale = torch.where(live, top / E4M3_MAX, 0.0)
     u = blocks * inv[:, None]
     if positive:
@@ -434,11 +432,6 @@ def _spread(blocked, flat, sizes):
     """The other way round, into the flat buffer."""
     padded = [k + (-k % BLOCK) for k in sizes]
     torch.cat([t[:k] for t, k in zip(blocked.split(padded), sizes)], out=flat)
-
-
-def _root(x):
-    """To nearest, by way of 64 bits: its codes lie next to borders too."""
-    return torch.sqrt(x.double()).float()
 
 
 def _plain_adamw(st):
@@ -463,7 +456,7 @@ def _plain_adamw(st):
     m = m * b1 + g * (1 - b1)
     v = v * b2 + (g * g) * (1 - b2)
     w = w * keep.repeat_interleave(count, output_size=w.numel())
-    w = w - (m / (_root(v * (1 / bc2)) + eps)) * (lr / bc1)
+    w = w - (m / (torch.sqrt(v * (1 / bc2)) + eps)) * (lr / bc1)
     if case["bits"] == 32:
         st["flat_p"].copy_(w)
         st["flat_m"].copy_(m)
@@ -471,7 +464,7 @@ def _plain_adamw(st):
         return
     _spread(w.to(DTYPES[case["dtype"]]), st["flat_p"], sizes)
     for x, c, sc, pos in ((m, "flat_m", "flat_ms", False),
-                          (_root(v), "flat_v", "flat_vs", True)):
+                          (torch.sqrt(v), "flat_v", "flat_vs", True)):
         codes, scales = _quantise(x, pos)
         _spread(codes.view(torch.uint8), st[c].view(torch.uint8), sizes)
         st[sc].copy_(scales)
