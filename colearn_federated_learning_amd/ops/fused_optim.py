@@ -226,12 +226,13 @@ def _quantise_(x: torch.Tensor, code: torch.Tensor, scale: torch.Tensor,
     blocks = _blocks(x)
     top = blocks.abs().nan_to_num(nan=0.0, posinf=float("inf")).amax(dim=1)
     live = top > _TINY
-    # a division: a number over a tensor would be a reciprocal's product
-    inv = torch.full_like(top, _E4M3_MAX) / top
+    # products with reciprocals, as the kernel's: a division by a number is one
+    # on the GPU, and none on the CPU
+    inv = top.reciprocal() * _E4M3_MAX
     u = blocks * torch.where(live, inv, 0.0)[:, None]
     if positive:
         u = torch.where(u > 0, u.clamp_min(_E4M3_MIN), u)
-    scale.copy_(torch.where(live, top / _E4M3_MAX, 0.0))
+    scale.copy_(torch.where(live, top * (1.0 / _E4M3_MAX), 0.0))
     code.view(-1).copy_(u.view(-1)[: x.numel()].to(code.dtype))
 
 

@@ -396,3 +396,54 @@ def test_refusals(dev):
         wide = torch.zeros(300, 2, device=dev)
         refuse(bad, [wide[:, 0], p[1]], g, m, v)  # strided
         refuse(bad, p, g, m, v, live=torch.ones(3, device=dev))
+
+
+def _plain_step(w, g, m, v, ms, vs, t, lr=1e-2, wd=0.1):
+    """One 8-bit step of one tensor of whole blocks, in fp32 operations of
+    torch: (w, m codes, v codes, m scales, v scales)."""
+    b1, b2 = 0.9, 0.999
+    bc1, bc2 = 1 - b1 ** t, 1 - b2 ** t
+    fm = (m.float().view(-1, 256) * ms[:, None]).view(-1)
+    fv = (v.float().view(-1, 256) * vs[:, None]).view(-1)
+    fm = fm * b1 + g * (1 - b1)
+    fv = (fv * fv) * b2 + (g * g) * (1 - b2)
+
+    def root(x):  # to nearest, on the CPU too
+        return torch.sqrt(x.double()).float()
+
+    w = w * (1 - lr * wd) - (fm / (root(fv * (1 / bc2)) + 1e-8)) * (lr / bc1)
+    held = []
+    for x in (fm, root(fv)):
+        top = x.view(-1, 256).abs().amax(1)
+        scale = top * (1 / 448)
+        inv = top.reciprocal() * 448
+        if x.is_cuda:  # what torch makes of these two
+            assert torch.equal(scale, top / 448)
+            assert torch.equal(inv, 448 / top)
+        u = x.view(-1, 256) * inv[:, None]
+        if x is not fm:
+            u = torch.where(u > 0, u.clamp_min(2.0 ** -9), u)
+        held.append((u.view(-1).to(torch.float8_e4m3fn), scale))
+    (m, ms), (v, vs) = held
+    return w, m, v, ms, vs
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("native", [True, False])
+def test_same_bits_as_plain_operations(dev, native, monkeypatch):
+    """Codes next to a border and all scales: over several steps, what
+    elementary operations of torch give on the same device."""
+    if not native:
+        monkeypatch.setenv("COLEARN_DISABLE_NATIVE", "1")
+    n = 256 * 8192
+    p = _tensors([(n,)], torch.float32, 0, 0.1)[0].to(dev)
+    want = [p.clone()]
+    m, v, ms, vs = adamw_state([p], 8)
+    want += [x[0].clone() for x in (m, v, ms, vs)]
+    for t in range(1, 5):
+        g = _tensors([(n,)], torch.float32, 10 + t, 0.01)[0].to(dev)
+        adamw_step([p], [g], m, v, exp_avg_scales=ms, exp_avg_sq_scales=vs,
+                   step=t, lr=1e-2, weight_decay=0.1)
+        want = _plain_step(want[0], g, *want[1:], t)
+        for a, b in zip((p, m[0], v[0], ms[0], vs[0]), want):
+            assert torch.equal(_codes(a), _codes(b))
