@@ -84,16 +84,14 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_dq_kernel(
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] -= delta;
+    sc.bend(z);
     if constexpr (M == kCap) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float th = fast_tanh(z[r] * sc.cap_in);
-        w[r] = 1.f - th * th;
-      }
+      for (int r = 0; r < 16; ++r) w[r] = 1.f - z[r] * z[r];
     }
     const float lane_part =
-        sc.c * sc.shape(z, static_cast<float>(own - t0 - other),
-                        own_wave - t0 - kb * 32) - lse + up;
+        sc.c * sc.lean(z, static_cast<float>(own - t0 - other),
+                       own_wave - t0 - kb * 32) - lse + up;
     if (mixed) mask<true>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
 #pragma unroll
     for (int r = 0; r < 16; ++r)
@@ -301,15 +299,13 @@ masked_attn_dkv_kernel(MaskedAttn a) {
         dp[g * 4 + 2] -= de.z;
         dp[g * 4 + 3] -= de.w;
       }
+      sc.bend(z);
       if constexpr (M == kCap) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float th = fast_tanh(z[r] * sc.cap_in);
-          dp[r] *= 1.f - th * th;
-        }
+        for (int r = 0; r < 16; ++r) dp[r] *= 1.f - z[r] * z[r];
       }
       const float up = fast_exp2(lift.log2() - kLift<T>);
-      sc.shape(z, static_cast<float>(own - t0 - other));
+      sc.lean(z, static_cast<float>(own - t0 - other));
       if (((cls >> (2 * i)) & 3) != 2)
         mask<false>(z, own_doc, lim, t0 + other, sm.doc[buf] + other);
 #pragma unroll

@@ -72,8 +72,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void masked_attn_fwd_kernel
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int other = t0 + i * 32 + 4 * half;
-      lane_part[i] = sc.c * sc.shape(z[i], static_cast<float>(own - other),
-                                     own_wave - t0 - i * 32);
+      sc.bend(z[i]);
+      lane_part[i] = sc.c * sc.lean(z[i], static_cast<float>(own - other),
+                                    own_wave - t0 - i * 32);
       // a half without any pair comes along as one whose pairs are all masked
       if (((cls >> (2 * i)) & 3) != 2)
         mask<true>(z[i], own_doc, lim, other, dt + i * 32 + 4 * half);

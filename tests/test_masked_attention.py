@@ -611,3 +611,46 @@ def test_functional_gradient():
     go = torch.randn(1, 70, 128, generator=g).to(torch.bfloat16).cuda()
     out, pull = torch.func.vjp(colearn_attention_qkv, x)
     _check_part(slice(0, 70), x, out, pull(go)[0], go)
+
+
+def _check_within_range(dev, s, h, hkv, d, dtype, std, **kw):
+    """As `_check`, for values that may not fit the type: what is past its
+    largest value has to be infinite, or that value, with the right sign."""
+    g = torch.Generator().manual_seed(s)
+    q, k, v, go = ((torch.randn(1, s, x, d, generator=g) * std).to(dtype)
+                   .to(dev).requires_grad_() for x in (h, hkv, hkv, h))
+    out = colearn_attention(q, k, v, **{
+        x: (y.to(dev) if torch.is_tensor(y) else y) for x, y in kw.items()})
+    got = (out, *torch.autograd.grad(out, (q, k, v), go))
+    most = torch.finfo(dtype).max
+    for name, x, y, t in zip(("out", "dq", "dk", "dv"), got,
+                             *_oracle(q, k, v, go, d ** -0.5, **kw)):
+        x = x.detach().cpu().double()
+        past = y.abs() + t > most
+        ok = (x - y).abs() <= t
+        ok |= past & (x.abs() >= most) & (x.sign() == y.sign())
+        assert ok.all(), f"{name}: {(~ok).sum()} of {ok.numel()}"
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("cap,std", [
+    (63.0, 1.5), (65.0, 1.5), (1e3, 1.5), (1e3, 16.0), (1e5, 1.5), (1e5, 64.0),
+    (1e8, 1.5), (1e18, 1.5)])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16),
+                                     (128, torch.float16)])
+def test_large_softcaps(dev, cap, std, d, dtype):
+    """Scores far below the cap keep their digits (std 16 and 64: scores of the
+    cap's size).  tanh is off by 4e-7 of itself and so is the score: within the
+    2^-17 (1 + max|z|) that the file's tolerances have for it."""
+    _check_within_range(dev, 260, 2, 2, d, dtype, std, softcap=cap,
+                        causal=True)
+    _check_within_range(dev, 150, 4, 2, d, dtype, std, softcap=cap,
+                        slopes=distance_slopes(4))
+
+
+@pytest.mark.gpu
+def test_large_softcaps_in_grids_that_fill_the_chip():
+    _check("cuda", 20, 257, 12, 12, 64, torch.bfloat16, packed=True,
+           softcap=1e6, slopes=distance_slopes(12), doc=_docs(20, 257, 6, 150))
+    _check("cuda", 8, 1090, 4, 4, 128, torch.float16, softcap=1e6, causal=True,
+           doc=_docs(8, 1090, 7, 800))
