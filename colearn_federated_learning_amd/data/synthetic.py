@@ -19,6 +19,8 @@ from ..utils.seed import stable_hash
 
 from ..config import DataConfig, ModelConfig
 
+MASK_TOKEN = 103  # what text_synth writes over the tokens to be guessed
+
 
 @dataclass
 class ClientShard:
@@ -86,15 +88,24 @@ def make_client_dataset(
         if v < 104:
             raise ValueError(
                 f"text_synth needs vocab_size >= 104 (the [MASK]-style "
-                f"token id is 103), got {v}")
+                f"token id is {MASK_TOKEN}), got {v}")
         lo = min(1000, v // 2)  # reserve low ids for special tokens
         ids = torch.randint(lo, v, (n, s), generator=gen)
         # MLM masking: select ~mlm_probability positions; label = original id
         mask = torch.rand(n, s, generator=gen) < data_cfg.mlm_probability
         mask[:, 0] = False  # keep a CLS-like position intact
+        # documents and padding are read from the masked ids
+        # (models.bert.document_ids): their tokens stay, and are not scored
+        for token in (model_cfg.doc_sep_token, model_cfg.pad_token):
+            if token == MASK_TOKEN:
+                raise ValueError(
+                    f"token {token} masks the others: it can neither end "
+                    f"documents nor pad")
+            if token is not None:
+                mask &= ids.ne(token)
         mlm_labels = torch.full((n, s), -100, dtype=torch.long)
         mlm_labels[mask] = ids[mask]
         ids = ids.clone()
-        ids[mask] = 103  # [MASK]-style token id
+        ids[mask] = MASK_TOKEN
         return ClientShard(ids, mlm_labels, client_id)
     raise ValueError(f"unknown dataset {data_cfg.dataset!r}")
