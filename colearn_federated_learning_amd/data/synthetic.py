@@ -53,6 +53,39 @@ def _class_means(num_classes: int, dim: int, gen: torch.Generator) -> torch.Tens
     return 1.5 * means / means.norm(dim=1, keepdim=True)
 
 
+def _write_documents(ids: torch.Tensor, data_cfg: DataConfig,
+                     model_cfg: ModelConfig, client_id: int) -> None:
+    """Where the model tells documents or padding apart, rows hold several
+    documents of an eighth to half a row, each ended by the separator, and end
+    in up to a quarter of padding.  In place; other rows are left alone, and
+    the caller's random numbers are not used."""
+    sep, pad = model_cfg.doc_sep_token, model_cfg.pad_token
+    n, s = ids.shape
+    for token in (sep, pad):
+        if token == MASK_TOKEN:
+            raise ValueError(
+                f"token {token} masks the others: it can neither end "
+                f"documents nor pad")
+        if token is not None and not 0 <= token < data_cfg.vocab_size:
+            raise ValueError(f"token {token} is not in a vocabulary of "
+                             f"{data_cfg.vocab_size}")
+    if sep is None and pad is None:
+        return
+    gen = torch.Generator().manual_seed(
+        stable_hash(data_cfg.seed, "documents", client_id))
+    fill = torch.full((n, 1), s)
+    if pad is not None:
+        fill = s - torch.randint(0, s // 4 + 1, (n, 1), generator=gen)
+    if sep is not None:
+        least = max(1, s // 8)
+        lens = torch.randint(least, max(least, s // 2) + 1, (n, -(-s // least)),
+                             generator=gen)
+        ends = torch.minimum(lens.cumsum(dim=1), fill) - 1
+        ids.scatter_(1, ends, sep)
+    if pad is not None:
+        ids.masked_fill_(torch.arange(s) >= fill, pad)
+
+
 def make_client_dataset(
     data_cfg: DataConfig, model_cfg: ModelConfig, client_id: int,
     labels: torch.Tensor,
@@ -91,16 +124,13 @@ def make_client_dataset(
                 f"token id is {MASK_TOKEN}), got {v}")
         lo = min(1000, v // 2)  # reserve low ids for special tokens
         ids = torch.randint(lo, v, (n, s), generator=gen)
+        _write_documents(ids, data_cfg, model_cfg, client_id)
         # MLM masking: select ~mlm_probability positions; label = original id
         mask = torch.rand(n, s, generator=gen) < data_cfg.mlm_probability
         mask[:, 0] = False  # keep a CLS-like position intact
         # documents and padding are read from the masked ids
         # (models.bert.document_ids): their tokens stay, and are not scored
         for token in (model_cfg.doc_sep_token, model_cfg.pad_token):
-            if token == MASK_TOKEN:
-                raise ValueError(
-                    f"token {token} masks the others: it can neither end "
-                    f"documents nor pad")
             if token is not None:
                 mask &= ids.ne(token)
         mlm_labels = torch.full((n, s), -100, dtype=torch.long)

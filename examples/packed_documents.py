@@ -1,5 +1,5 @@
 """BERT masked-LM federated session over rows that hold several documents:
-a separator token ends each, attention stays within it, positions count by
+a separator token ends each, attention stays within it and falls off with
 distance, and AdamW holds its states in 8 bits.  Small CPU version; on MI355X
 attention, norms and the optimizer step run as HIP kernels.
 """

@@ -369,3 +369,39 @@ def test_the_masking_token_is_no_separator():
     for model in (dict(doc_sep_token=103), dict(pad_token=103)):
         with pytest.raises(ValueError, match="103"):
             _text(**model)
+
+
+def test_text_holds_documents_and_padding():
+    """At BERT's own vocabulary, with tokens below those that texts draw."""
+    for seq in (1, 2, 7, 17, 48, 128):
+        x, y, bert = _text(n=64, seq=seq, vocab=30522, doc_sep_token=102,
+                           pad_token=0)
+        doc = document_ids(x, bert)
+        live = doc >= 0
+        # padding at the end only, of a quarter at most
+        assert (live[:, 1:] <= live[:, :-1]).all()
+        assert live.sum(1).min() >= seq - seq // 4
+        # every document is ended, the last one of a row with the row
+        last = live.sum(1, keepdim=True) - 1
+        assert x.gather(1, last).eq(102).all()
+        lens = [r[r >= 0].bincount() for r in doc]
+        least = max(1, seq // 8)
+        assert all((k[:-1] >= least).all() and k.max() <= max(1, seq // 2)
+                   for k in lens)
+        if seq >= 48:
+            assert all(len(k) >= 2 for k in lens) and not live.all()
+    # either alone; and neither changes the tokens that remain
+    plain, _, _ = _text(n=64, seq=48, vocab=30522)
+    sep, _, _ = _text(n=64, seq=48, vocab=30522, doc_sep_token=102)
+    pad, _, _ = _text(n=64, seq=48, vocab=30522, pad_token=0)
+    assert not plain.eq(102).any() and not plain.eq(0).any()
+    assert (sep.eq(plain) | sep.eq(102) | plain.eq(103)).all()
+    assert (pad.eq(plain) | pad.eq(0) | plain.eq(103)).all()
+    assert sep.eq(102).sum() >= 2 * 64 and pad.eq(0).any()
+
+
+@pytest.mark.parametrize("token", [-1, 128])
+def test_tokens_outside_the_vocabulary_are_refused(token):
+    for name in ("doc_sep_token", "pad_token"):
+        with pytest.raises(ValueError, match="vocabulary"):
+            _text(**{name: token})
