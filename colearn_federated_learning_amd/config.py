@@ -20,7 +20,8 @@ class DataConfig:
     """Synthetic dataset shape + federated sharding."""
 
     dataset: str = "mnist_synth"  # mnist_synth | cifar10_synth | text_synth | file
-    # dataset="file": torch.save'd {"x": [N,C,H,W] float, "y": [N] int64}
+    # dataset="file": torch.save'd {"x": [N,C,H,W] float, "y": [N] int64}, or
+    # {"x": token ids [N,S], "y": masked-LM labels [N,S]}
     # partitioned across clients by the same IID/Dirichlet axes (data/files.py)
     data_path: Optional[str] = None
     num_classes: int = 10

@@ -6,6 +6,9 @@ equivalent capability here is ``dataset: "file"``: a ``torch.save``d dict
 ``{"x": float tensor [N,C,H,W], "y": int64 [N]}`` (or an (x, y) tuple) is
 partitioned across clients with the same IID / Dirichlet(alpha) label-skew
 axes as the synthetic sharder — on REAL samples, by index assignment.
+Text for masked-LM training is ``{"x": token ids [N,S], "y": labels [N,S]}``,
+both integers (-100 where a token is not scored); it has no label skew and
+is partitioned IID.
 
 Determinism contract matches data/sharder.py: the partition depends only
 on (seed, num_clients, client_id, file labels), never on rank layout.
@@ -31,7 +34,11 @@ def load_file_dataset(path: str) -> Tuple[torch.Tensor, torch.Tensor]:
             x, y = obj["x"], obj["y"]
         else:
             x, y = obj
-        _CACHE[path] = (x.float(), y.long())
+        # token ids keep their type: labels of every position tell them from
+        # integer features
+        text = (x.dim() == 2 and x.shape == y.shape
+                and not (x.is_floating_point() or y.is_floating_point()))
+        _CACHE[path] = (x.long() if text else x.float(), y.long())
     return _CACHE[path]
 
 
@@ -60,6 +67,9 @@ def partition_file_indices(
         return [perm[i * per : (i + 1) * per] for i in range(num_clients)]
     if cfg.partition != "dirichlet":
         raise ValueError(f"unknown partition {cfg.partition!r}")
+    if y.dim() != 1:
+        raise ValueError("a dirichlet partition needs one label a sample, got "
+                         f"labels {tuple(y.shape)}")
     # per-class index pools, shuffled once with the global seed
     g = torch.Generator().manual_seed(stable_hash(cfg.seed, "file_dir"))
     classes = sorted(int(c) for c in torch.unique(y))

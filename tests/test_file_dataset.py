@@ -1,5 +1,6 @@
 """dataset="file": real-data loading + federated partitioning."""
 
+import pytest
 import torch
 
 from colearn_federated_learning_amd import driver_config, run
@@ -108,3 +109,41 @@ def test_whole_dataset_split(tmp_path):
     assert all(len(q) == 25 for q in parts)
     allidx = torch.cat(parts)
     assert torch.unique(allidx).numel() == 100
+
+
+def test_packed_text_from_a_file_reaches_bert(tmp_path):
+    """Token ids and a label a position: they stay integers, documents and
+    all."""
+    g = torch.Generator().manual_seed(0)
+    y = torch.randint(10, 64, (24, 32), generator=g)
+    x = y.clone()
+    x[:, 15] = 9
+    scored = torch.rand(24, 32, generator=g) < 0.3
+    scored[:, 15] = False
+    y[~scored] = -100
+    x[scored] = 8
+    p = tmp_path / "text.pt"
+    torch.save({"x": x.int(), "y": y.int()}, p)
+    cfg = driver_config(4).override(
+        data__dataset="file", data__data_path=str(p), data__seq_len=32,
+        data__samples_per_client=12, data__vocab_size=64, rounds=1,
+        num_clients=2, train__batch_size=4, train__dtype="float32",
+        model__hidden_size=32, model__num_layers=1, model__num_heads=2,
+        model__intermediate_size=32, model__doc_sep_token=9,
+        model__attn_dropout=0.0, model__dropout=0.0)
+    shards = make_shards(cfg.data, 2)
+    assert sorted(torch.cat(shards).tolist()) == list(range(24))
+    shard = make_client_dataset(cfg.data, cfg.model, 1, shards[1])
+    assert shard.x.dtype == shard.y.dtype == torch.long
+    assert torch.equal(shard.x, x[shards[1]])
+    (rec,) = run(cfg)
+    assert rec["mean_client_loss"] == rec["mean_client_loss"]
+    with pytest.raises(ValueError, match="one label a sample"):
+        make_shards(cfg.override(data__partition="dirichlet").data, 2)
+
+
+def test_integer_features_are_still_floats(tmp_path):
+    p = tmp_path / "bytes.pt"
+    torch.save({"x": torch.ones(6, 1, 2, 2, dtype=torch.uint8),
+                "y": torch.zeros(6, dtype=torch.long)}, p)
+    assert load_file_dataset(str(p))[0].dtype == torch.float32
