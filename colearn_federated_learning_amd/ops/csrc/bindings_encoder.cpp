@@ -314,13 +314,15 @@ torch::Tensor add_norm_bwd(torch::Tensor gy, OptTensor gs, torch::Tensor s,
 
 // ---- masked attention ---------------------------------------------------------
 // The kernels read 16 bytes at a time: rows of contiguous elements whose
-// strides and start are multiples of 8 of them.  Anything else is copied.
+// strides and start are multiples of 8 of them.  Anything else is copied
+// (`contiguous` would return a contiguous tensor that starts off 16 bytes as it
+// is).
 torch::Tensor readable(const torch::Tensor& t) {
   bool ok = t.stride(3) == 1 && aligned16(t);
   for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
   // a tile's rows are addressed with 32 bits
   ok = ok && t.stride(1) >= 0 && t.stride(1) <= (1 << 23);
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 HeadView view_of(const torch::Tensor& t) {

@@ -654,3 +654,41 @@ def test_large_softcaps_in_grids_that_fill_the_chip():
            softcap=1e6, slopes=distance_slopes(12), doc=_docs(20, 257, 6, 150))
     _check("cuda", 8, 1090, 4, 4, 128, torch.float16, softcap=1e6, causal=True,
            doc=_docs(8, 1090, 7, 800))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [1, 3, 4])
+def test_operands_that_start_off_16_bytes(off):
+    """Contiguous views at odd elements of a flat buffer, each operand and the
+    output's gradient, with values on both sides that no result may show."""
+    g = torch.Generator().manual_seed(0)
+    doc = _docs(2, 150, 3, 60).cuda()
+    near = [torch.randn(2, 150, h, 64, generator=g).to(torch.bfloat16).cuda()
+            for h in (4, 2, 2, 4)]
+
+    def moved(t):
+        flat = torch.full((t.numel() + 16,), math.nan, dtype=t.dtype,
+                          device="cuda")
+        view = flat[off:off + t.numel()].view(t.shape)
+        assert view.is_contiguous() and view.data_ptr() % 16
+        return view.copy_(t)
+
+    def run(q, k, v, go):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        out = colearn_attention(q, k, v, doc=doc, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, (q, k, v), go)]
+
+    want = run(*near)
+    for i in range(4):
+        got = run(*(moved(t) if i == j else t for j, t in enumerate(near)))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = run(*(moved(t) for t in near))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    qkv = torch.randn(2, 150, 3, 4, 64, generator=g).to(torch.bfloat16).cuda()
+    res = []
+    for x, go in ((qkv, near[3]), (moved(qkv), moved(near[3]))):
+        x = x.detach().requires_grad_()
+        out = colearn_attention_qkv(x, doc=doc)
+        res.append([out.detach(),
+                    *torch.autograd.grad(out, x, go.view(2, 150, 256))])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
