@@ -313,6 +313,8 @@ torch::Tensor add_norm_bwd(torch::Tensor gy, OptTensor gs, torch::Tensor s,
 }
 
 // ---- masked attention ---------------------------------------------------------
+constexpr int64_t kMostRow = 1 << 23;  // elements from a token to the next
+
 // The kernels read 16 bytes at a time: rows of contiguous elements whose
 // strides and start are multiples of 8 of them.  Anything else is copied
 // (`contiguous` would return a contiguous tensor that starts off 16 bytes as it
@@ -320,8 +322,8 @@ torch::Tensor add_norm_bwd(torch::Tensor gy, OptTensor gs, torch::Tensor s,
 torch::Tensor readable(const torch::Tensor& t) {
   bool ok = t.stride(3) == 1 && aligned16(t);
   for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
-  // a tile's rows are addressed with 32 bits
-  ok = ok && t.stride(1) >= 0 && t.stride(1) <= (1 << 23);
+  // a tile's rows are addressed with 32 bits (a copy's are: `describe`)
+  ok = ok && t.stride(1) >= 0 && t.stride(1) <= kMostRow;
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -365,6 +367,8 @@ MaskedAttn describe(const torch::Tensor& q, const torch::Tensor& k,
           N * H * ((S + 63) / 64) <= kMostBlocks,
       "attention: too many tokens (a sequence has at most 2^22, all heads of "
       "all sequences 2^24 tiles of 64)");
+  TORCH_CHECK_VALUE(H * D <= kMostRow, "attention: all heads of a token have "
+                    "at most ", kMostRow, " elements, not ", H * D);
   // the kernels form scale / softcap and slope / scale in fp32
   TORCH_CHECK_VALUE(scale >= 1e-18 && scale <= 1e18,
                     "attention: the scale must be within 1e-18 and 1e18, got ",

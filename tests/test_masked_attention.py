@@ -692,3 +692,23 @@ def test_operands_that_start_off_16_bytes(off):
         res.append([out.detach(),
                     *torch.autograd.grad(out, x, go.view(2, 150, 256))])
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.gpu
+def test_tokens_of_more_than_32_bits_a_tile_are_refused():
+    """A tile's 64 rows are addressed with 32 bits: tokens of 2^23 elements are
+    the largest, whether read as they are or copied."""
+    def rows(h):  # 64 KB, whatever its shape says
+        return torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16,
+                           device="cuda").expand(1, 1, h, 128)
+
+    for h in (2 ** 16 + 1, 2 ** 18 + 1):
+        with pytest.raises(ValueError, match="8388608"):
+            colearn_attention(rows(h), rows(h), rows(h))
+        with pytest.raises(ValueError, match="8388608"):
+            colearn_attention(rows(h), rows(1), rows(1))
+    x = torch.randn(1, 3, 2 ** 16, 128, device="cuda").to(torch.bfloat16)
+    out = colearn_attention(x, x, x)
+    for part in (slice(0, 4), slice(2 ** 16 - 4, 2 ** 16)):
+        few = x[:, :, part].contiguous()
+        assert torch.equal(out[:, :, part], colearn_attention(few, few, few))
