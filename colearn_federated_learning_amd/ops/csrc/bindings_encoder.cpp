@@ -122,6 +122,10 @@ void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
       check(vs[i], torch::kFloat32, blocks, true, "a second moment's scales");
     }
     if (prox) check(ref[i], torch::kFloat32, n, false, "a reference");
+    // as many elements in another order would be another tensor's step
+    for (const auto* t : {&g[i], &m[i], &v[i], prox ? &ref[i] : &p[i]})
+      TORCH_CHECK_VALUE(t->sizes() == p[i].sizes(), "adamw: ", t->sizes(),
+                        " beside a parameter ", p[i].sizes());
   }
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i)

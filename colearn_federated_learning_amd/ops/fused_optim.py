@@ -262,7 +262,8 @@ def adamw_step(
     gradient is None are left out.
 
     Parameters are all float32 or all bfloat16 (rounded to nearest), and so
-    are gradients; everything is contiguous and on one device, and no tensor
+    are gradients; gradients, moments and references have their parameter's
+    shape; everything is contiguous and on one device, and no tensor
     that is written may overlap another operand.  ``live``: float32 ``[lr / bc1,
     1 / bc2]`` on the device, read by the kernel in place of what ``step`` and
     ``lr`` give (a captured graph's arguments are frozen).
@@ -305,10 +306,12 @@ def adamw_step(
     if any(t.dtype not in (torch.float32, torch.bfloat16) for t in ps + gs):
         raise TypeError("parameters and gradients must be float32 or "
                         "bfloat16")
+    for ts in (gs, ms, vs, rs or ps):
+        for p, t in zip(ps, ts):
+            if t.shape != p.shape:
+                raise ValueError(f"{tuple(t.shape)} beside a parameter "
+                                 f"{tuple(p.shape)}")
     for i, (p, g) in enumerate(zip(ps, gs)):
-        if g.shape != p.shape:
-            raise ValueError(f"gradient {tuple(g.shape)} of a parameter "
-                             f"{tuple(p.shape)}")
         w, gw = p.float().reshape(-1), g.float().reshape(-1)
         if rs is not None:
             gw = gw + (w - rs[i].reshape(-1)) * fedprox_mu

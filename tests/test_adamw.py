@@ -447,3 +447,27 @@ def test_same_bits_as_plain_operations(dev, native, monkeypatch):
         want = _plain_step(want[0], g, *want[1:], t)
         for a, b in zip((p, m[0], v[0], ms[0], vs[0]), want):
             assert torch.equal(_codes(a), _codes(b))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("which", ["gradient", "first moment",
+                                   "second moment", "reference"])
+def test_another_shape_is_refused(dev, bits, which):
+    """As many elements, contiguous, in another order; nothing is written."""
+    p = torch.ones(16, 32, device=dev)
+    m, v, ms, vs = adamw_state([p], bits)
+    ops = [torch.ones_like(p), m[0], v[0], torch.zeros_like(p)]
+    i = ["gradient", "first moment", "second moment",
+         "reference"].index(which)
+    for shape in ((32, 16), (512,)):
+        bad = list(ops)
+        bad[i] = bad[i].view(shape)
+        with pytest.raises(ValueError, match="beside a parameter"):
+            adamw_step([p], [bad[0]], [bad[1]], [bad[2]], exp_avg_scales=ms,
+                       exp_avg_sq_scales=vs, step=1, lr=0.1, fedprox_mu=0.1,
+                       refs=[bad[3]])
+    assert (p == 1).all() and not any(_codes(t).any() for t in (m[0], v[0]))
+    adamw_step([p], [ops[0]], m, v, exp_avg_scales=ms, exp_avg_sq_scales=vs,
+               step=1, lr=0.1, fedprox_mu=0.1, refs=[ops[3]])
+    assert (p != 1).all()
