@@ -630,7 +630,7 @@ template <bool OWN_Q>
 DEV_INLINE int pair_limit(const MaskedAttn& a, int n, int own) {
   if (!a.causal) return OWN_Q ? 0x7fffffff : 0;
   const int prefix = a.prefix != nullptr ? a.prefix[n] : 0;
-  if (OWN_Q) return max(own, prefix - 1);
+  if (OWN_Q) return max(own, max(prefix, 0) - 1);
   return own < prefix ? 0 : own;
 }
 

@@ -712,3 +712,12 @@ def test_tokens_of_more_than_32_bits_a_tile_are_refused():
     for part in (slice(0, 4), slice(2 ** 16 - 4, 2 ** 16)):
         few = x[:, :, part].contiguous()
         assert torch.equal(out[:, :, part], colearn_attention(few, few, few))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_prefixes_at_the_ends_of_the_type(dev):
+    prefix = torch.tensor([-2 ** 31, -2 ** 31 + 1, 2 ** 31 - 1],
+                          dtype=torch.int32)
+    for s in (40, 200):
+        _check(dev, 3, s, 2, 2, 64, torch.bfloat16, seed=s, causal=True,
+               prefix=prefix)
