@@ -271,9 +271,11 @@ def adamw_step(
     b1, b2 = betas
     if step < 1 and live is None:
         raise ValueError(f"step counts from 1, got {step}")
-    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps > 0.0):
-        raise ValueError(f"betas must be in [0, 1) and eps positive, got "
-                         f"{betas}, {eps}")
+    # eps is added in float32: one below its smallest value would be lost, and
+    # a weight without gradients divided by zero
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 2.0 ** -149):
+        raise ValueError(f"betas must be in [0, 1) and eps positive in "
+                         f"float32, got {betas}, {eps}")
     if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
         raise ValueError("scales of both moments, or of none")
     if (refs is None) != (fedprox_mu == 0.0):

@@ -471,3 +471,19 @@ def test_another_shape_is_refused(dev, bits, which):
     adamw_step([p], [ops[0]], m, v, exp_avg_scales=ms, exp_avg_sq_scales=vs,
                step=1, lr=0.1, fedprox_mu=0.1, refs=[ops[3]])
     assert (p != 1).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_an_eps_that_float32_loses_is_refused(dev, bits):
+    """Zero gradients over an eps of 0 would be NaN."""
+    p = [torch.ones(300, device=dev)]
+    m, v, ms, vs = adamw_state(p, bits)
+    kw = dict(exp_avg_scales=ms, exp_avg_sq_scales=vs, step=1, lr=0.1,
+              weight_decay=0.0)
+    for eps in (1e-50, 2.0 ** -151, math.nan):
+        with pytest.raises(ValueError, match="eps"):
+            adamw_step(p, [torch.zeros_like(p[0])], m, v, eps=eps, **kw)
+    for eps in (2.0 ** -149, 1e-30):
+        adamw_step(p, [torch.zeros_like(p[0])], m, v, eps=eps, **kw)
+        assert (p[0] == 1).all()
