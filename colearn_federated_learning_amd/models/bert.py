@@ -112,8 +112,13 @@ class MaskedAttentionMixin:
             slopes = self._slopes
             if slopes is None or slopes.device != qkv.device:
                 slopes = distance_slopes(self.h, qkv.device)
-                # not one that lives in a transform or is closed to autograd
-                if not (is_vmapped() or torch.is_inference_mode_enabled()):
+                # not one that lives in a transform, is closed to autograd, or
+                # belongs to a graph that has yet to be replayed
+                if not (is_vmapped() or torch.is_inference_mode_enabled()
+                        or (qkv.is_cuda
+                            and torch.cuda.is_current_stream_capturing())):
+                    if qkv.is_cuda:  # there, whichever stream asks next
+                        torch.cuda.current_stream(qkv.device).synchronize()
                     self._slopes = slopes
         return colearn_attention_qkv(qkv, doc=doc, softcap=self.softcap,
                                      slopes=slopes)

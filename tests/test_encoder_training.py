@@ -11,7 +11,7 @@ import torch
 from colearn_federated_learning_amd import FederatedServer, driver_config
 from colearn_federated_learning_amd.data.synthetic import make_client_dataset
 from colearn_federated_learning_amd.models.bert import (
-    BertConfig, BertForMaskedLM, document_ids)
+    BertConfig, BertForMaskedLM, BertSelfAttention, document_ids)
 from colearn_federated_learning_amd.ops.attention import (
     colearn_attention_qkv, distance_slopes)
 from colearn_federated_learning_amd.ops.fused_optim import (
@@ -405,3 +405,31 @@ def test_tokens_outside_the_vocabulary_are_refused(token):
     for name in ("doc_sep_token", "pad_token"):
         with pytest.raises(ValueError, match="vocabulary"):
             _text(**{name: token})
+
+
+@pytest.mark.gpu
+def test_attention_first_used_in_a_graph():
+    """The distance slopes that a capture makes are the graph's own: eager work
+    before its first replay, or on another stream, has slopes of its own."""
+    torch.manual_seed(0)
+    cfg = BertConfig(hidden_size=64, num_heads=2, attn_distance_bias=True,
+                     attn_dropout=0.0)
+    warm, attn = (BertSelfAttention(cfg).cuda() for _ in range(2))
+    x = torch.randn(2, 90, 3, 2, 32, device="cuda").to(torch.bfloat16)
+    want = warm._masked_attention(x, None)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = attn._masked_attention(x, None)
+    assert attn._slopes is None
+    assert torch.equal(attn._masked_attention(x, None), want)
+    kept = attn._slopes
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert torch.equal(attn._masked_attention(x, None), want)
+    for _ in range(3):
+        out.zero_()
+        gr.replay()
+        attn._masked_attention(x, None)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert attn._slopes is kept
