@@ -304,7 +304,7 @@ def adamw_step(
         return
     up, inv_bc2 = lr / bc1, 1.0 / bc2
     if live is not None:
-        up, inv_bc2 = (float(x) for x in live)
+        up, inv_bc2 = live.unbind()  # not read by the host: may be captured
     if any(t.dtype not in (torch.float32, torch.bfloat16) for t in ps + gs):
         raise TypeError("parameters and gradients must be float32 or "
                         "bfloat16")

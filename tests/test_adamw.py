@@ -487,3 +487,54 @@ def test_an_eps_that_float32_loses_is_refused(dev, bits):
     for eps in (2.0 ** -149, 1e-30):
         adamw_step(p, [torch.zeros_like(p[0])], m, v, eps=eps, **kw)
         assert (p[0] == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_the_torch_path_is_captured_too(bits, monkeypatch):
+    """With the kernels switched off, what a captured step reads at a replay is
+    the live scalars, as with them."""
+    segs = [(500, True), (37, False), (4000, True)]
+    n = sum(k for k, _ in segs)
+    start = _tensors([(n,)], torch.float32, 0, 0.1)[0].cuda()
+    grads = [t.cuda() for t in _tensors([(n,)] * 4, torch.float32, 1, 0.1)]
+
+    def make():
+        w, g = start.clone(), torch.zeros_like(start)
+        return FlatAdamW(w, g, lr=0.1, state_bits=bits, segments=segs), w, g
+
+    eager, we, ge = make()
+    opt, w, g = make()
+    with monkeypatch.context() as off:
+        off.setenv("COLEARN_DISABLE_NATIVE", "1")
+        opt.host_prepare()
+        opt.device_step()  # warm
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            opt.device_step()
+    w.copy_(start)
+    opt.reset()
+    for x in grads:
+        ge.copy_(x)
+        eager.step()  # the kernel: the same bits
+        g.copy_(x)
+        opt.host_prepare()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, we)
+        for a, b in zip(opt.m + opt.v, eager.m + eager.v):
+            assert torch.equal(_codes(a), _codes(b))
+
+
+def test_live_scalars_on_the_cpu():
+    res = []
+    for live in (None, torch.tensor([0.1 / (1 - 0.9 ** 3),
+                                     1 / (1 - 0.999 ** 3)])):
+        p = _tensors([(300,)], torch.float32, 0, 0.1)
+        m, v, ms, vs = adamw_state(p, 8)
+        adamw_step(p, _tensors([(300,)], torch.float32, 1, 0.1), m, v,
+                   exp_avg_scales=ms, exp_avg_sq_scales=vs,
+                   step=3 if live is None else 1, lr=0.1, live=live)
+        res.append([p[0], _codes(m[0]), _codes(v[0])])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
