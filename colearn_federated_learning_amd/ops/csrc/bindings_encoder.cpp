@@ -71,6 +71,14 @@ bool aligned16(const torch::Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// no byte of either contiguous tensor is the other's
+bool apart(const torch::Tensor& a, const torch::Tensor& b) {
+  const auto at = [](const torch::Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr());
+  };
+  return at(a) + a.nbytes() <= at(b) || at(b) + b.nbytes() <= at(a);
+}
+
 // ---- AdamW ------------------------------------------------------------------
 void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
                 std::vector<torch::Tensor> m, std::vector<torch::Tensor> v,
@@ -615,7 +623,13 @@ std::tuple<torch::Tensor, torch::Tensor> add_layer_norm(
                     g->numel() == weight.numel(),
                 "add_norm: gradient slots must be contiguous float32 of "
                 "weight's size");
+    // one launch writes both, column by column
+    TORCH_CHECK(apart(*g, weight) && apart(*g, bias),
+                "add_norm: gradient slots must not overlap the parameters");
   }
+  TORCH_CHECK(!gslot_w.has_value() || !gslot_b.has_value() ||
+                  apart(*gslot_w, *gslot_b),
+              "add_norm: gradient slots must not overlap each other");
   auto out = AddNormFn::apply(x, residual, weight, bias, eps, groups, gslot_w,
                               gslot_b);
   return {out[0], out[1]};

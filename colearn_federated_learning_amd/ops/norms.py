@@ -307,8 +307,9 @@ def colearn_add_layer_norm(
 
     ``groups`` > 1: stacked clients, rows client-major, ``weight`` and ``bias``
     [groups, H].  ``gslot_w`` / ``gslot_b`` (both or none, float32, weight's
-    size, contiguous): the backward writes the parameters' gradients there
-    (overwriting them) and returns none, as the stacked engine's norms do.
+    size, contiguous, apart from each other and from the parameters): the
+    backward writes the parameters' gradients there (overwriting them) and
+    returns none, as the stacked engine's norms do.
 
     float32, bfloat16 and float16 on the GPU, rows up to 16384, run the HIP
     kernels (csrc/add_norm.hip; up to 2^26 rows of 1024, 2^24 of 4096, 2^22 of

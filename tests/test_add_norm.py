@@ -338,3 +338,20 @@ def test_empty(dev):
     y.sum().backward()
     assert y.shape == s.shape == x.grad.shape == (0, 8)
     assert (w.grad == 0).all()
+
+
+@pytest.mark.gpu
+def test_slots_that_overlap_are_refused():
+    x = torch.zeros(6, 8, device="cuda", requires_grad=True)
+    flat = torch.ones(40, device="cuda")
+    w, b, slot = flat[:8], flat[8:16], flat[16:24]
+    for bad in (slot, flat[20:28], flat[12:20], w, b, flat[4:12]):
+        for pair in ((slot, bad), (bad, slot)):
+            with pytest.raises(RuntimeError, match="overlap"):
+                colearn_add_layer_norm(x, None, w, b, gslot_w=pair[0],
+                                       gslot_b=pair[1])
+    y, _ = colearn_add_layer_norm(x, None, w, b, gslot_w=slot,
+                                  gslot_b=flat[24:32])
+    y.sum().backward()
+    assert (flat[24:32] == 6).all() and (flat[16:24] == 0).all()
+    assert (flat[:16] == 1).all() and (flat[32:] == 1).all()
