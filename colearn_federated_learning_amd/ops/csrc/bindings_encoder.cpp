@@ -162,6 +162,10 @@ void adamw_step(std::vector<torch::Tensor> p, std::vector<torch::Tensor> g,
     TORCH_CHECK(live->scalar_type() == torch::kFloat32 &&
                     live->is_contiguous() && live->numel() == 2,
                 "adamw: the live scalars are two contiguous float32");
+    for (const auto* ts : {&p, &m, &v, &ms, &vs})
+      for (const auto& t : *ts)
+        TORCH_CHECK(apart(*live, t), "adamw: the live scalars overlap a tensor "
+                    "that the step writes");
     sc.live = live->data_ptr<float>();
   }
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);

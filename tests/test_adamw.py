@@ -538,3 +538,19 @@ def test_live_scalars_on_the_cpu():
                    step=3 if live is None else 1, lr=0.1, live=live)
         res.append([p[0], _codes(m[0]), _codes(v[0])])
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_live_scalars_that_the_step_writes_are_refused(bits):
+    p = [torch.ones(300, device="cuda") for _ in range(2)]
+    g = [torch.ones_like(x) for x in p]
+    m, v, ms, vs = adamw_state(p, bits)
+    kw = dict(exp_avg_scales=ms, exp_avg_sq_scales=vs, step=1, lr=0.1)
+    for live in [p[0][4:6], p[1][-2:]] + ([vs[1]] if bits == 8 else
+                                          [m[0][:2], v[1][-2:]]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            adamw_step(p, g, m, v, live=live, **kw)
+    assert all((x == 1).all() for x in p)
+    adamw_step(p, g, m, v, live=g[0][:2], **kw)
+    assert all((x < 1).all() for x in p)
