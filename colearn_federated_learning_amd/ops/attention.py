@@ -2,7 +2,8 @@
 
 ``colearn_attention`` / ``colearn_attention_qkv``: any length, with document
 masks and padding, causal and prefix masks, capped scores, linear distance
-biases and shared key heads (csrc/masked_attn.hip).
+biases and shared key heads (csrc/masked_attn.h, masked_attn_fwd.hip,
+masked_attn_bwd.hip).
 
 ``fused_attention``: unmasked, with dropout (BERT shapes: seq 128, dh = 64).
 

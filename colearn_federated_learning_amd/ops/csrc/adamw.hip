@@ -28,8 +28,8 @@
 // Bound by memory: 28 bytes an element with fp32 states, 16 with 8-bit ones.
 // A wave owns a block (four elements a lane), so a block's maximum is a wave
 // reduction and nothing goes through LDS.  One block a wave and nothing left to
-// wait for: BERT-base's 153 tensors, 110 M parameters, take 579 us with fp32
-// states (5.3 TB/s) and 321 us with 8-bit ones (5.5 TB/s) in four launches; two
+// wait for: BERT-base's 153 tensors, 110 M parameters, take 578 us with fp32
+// states (5.3 TB/s) and 317 us with 8-bit ones (5.5 TB/s) in four launches; two
 // blocks a wave, one after another, take 594 and 350 us.
 
 #include "elem.h"

@@ -185,8 +185,9 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void add_norm_bwd_kernel(
               (W == 1 ? threadIdx.x / kWave : 0);
   // The next rows' loads are under way while a row is reduced and written: two
   // rows of 16-bit elements (65536 x 768 in 8 groups 58 us, one row 63; 8192 x
-  // 4096 37 and 41), one of 32-bit ones (4099 x 1023 21, two 24), none where 16
-  // waves leave no registers for them.
+  // 4096 37 and 41), one of 32-bit ones (4099 x 1023, both gradients, 25.0, two
+  // 25.4; without the sum's 13.3, 13.8), none where 16 waves leave no registers
+  // for them.
   constexpr int kAhead = W == 16 ? 0 : sizeof(T) == 2 ? 2 : 1;
   struct Row {
     Raw<T, VEC> g[NV], s[NV];

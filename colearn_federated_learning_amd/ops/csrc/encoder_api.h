@@ -1,5 +1,5 @@
 // Launchers of the encoder-training kernels (adamw.hip, add_norm.hip,
-// masked_attn.hip), shared with bindings_encoder.cpp.
+// masked_attn_fwd.hip, masked_attn_bwd.hip), shared with bindings_encoder.cpp.
 #pragma once
 
 #include <hip/hip_runtime_api.h>

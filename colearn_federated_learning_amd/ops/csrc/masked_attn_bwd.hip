@@ -510,8 +510,8 @@ struct Backward {
 int masked_attn_shares(const MaskedAttn& a) {
   // Key heads that serve several heads leave the dk/dv grid short: the group
   // is shared out until there are two workgroups a CU, or every head has its
-  // own.  2 x 1999 capped tokens, 16 heads over 4, size 128: with the join, 281
-  // us in one share, 255 in two, 246 in four.
+  // own.  2 x 1999 capped tokens, 16 heads over 4, size 128: with the join, 292
+  // us in one share, 216 in two, 213 in four.
   const int group = a.H / a.Hkv;
   const int64_t blocks =
       static_cast<int64_t>(a.N) * a.Hkv * ((a.S + 127) / 128);
