@@ -172,7 +172,7 @@ def colearn_attention(
 
     Gradients of q, k and v are bitwise the same from run to run.  bfloat16 and
     float16 operands on the GPU with D a multiple of 8 up to 128 run the HIP
-    kernels (up to 2^23 elements a token over all heads; rows may be strided; a
+    kernels (up to 2^25 elements a token over all heads; rows may be strided; a
     last dimension that is not contiguous, or rows that do not start at 16
     bytes, are copied first); other operands run the same formulas in torch.
     Under autocast operands are cast first.

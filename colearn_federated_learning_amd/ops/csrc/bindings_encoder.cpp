@@ -329,7 +329,9 @@ torch::Tensor add_norm_bwd(torch::Tensor gy, OptTensor gs, torch::Tensor s,
 }
 
 // ---- masked attention ---------------------------------------------------------
-constexpr int64_t kMostRow = 1 << 23;  // elements from a token to the next
+// Elements from a token to the next.  A tile's 64 rows are addressed with 32
+// bits of bytes: 63 x 2^25 x 2 and a row's 256 are less than 2^32.
+constexpr int64_t kMostRow = 1 << 25;
 
 // The kernels read 16 bytes at a time: rows of contiguous elements whose
 // strides and start are multiples of 8 of them.  Anything else is copied
@@ -338,7 +340,7 @@ constexpr int64_t kMostRow = 1 << 23;  // elements from a token to the next
 torch::Tensor readable(const torch::Tensor& t) {
   bool ok = t.stride(3) == 1 && aligned16(t);
   for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
-  // a tile's rows are addressed with 32 bits (a copy's are: `describe`)
+  // a copy's tokens are not further apart: `describe`
   ok = ok && t.stride(1) >= 0 && t.stride(1) <= kMostRow;
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }

@@ -696,20 +696,30 @@ def test_operands_that_start_off_16_bytes(off):
 
 @pytest.mark.gpu
 def test_tokens_of_more_than_32_bits_a_tile_are_refused():
-    """A tile's 64 rows are addressed with 32 bits: tokens of 2^23 elements are
+    """A tile's 64 rows are addressed with 32 bits: tokens of 2^25 elements are
     the largest, whether read as they are or copied."""
-    def rows(h):  # 64 KB, whatever its shape says
+    def rows(h):  # 256 bytes, whatever the shape says
         return torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16,
                            device="cuda").expand(1, 1, h, 128)
 
-    for h in (2 ** 16 + 1, 2 ** 18 + 1):
-        with pytest.raises(ValueError, match="8388608"):
+    for h in (2 ** 18 + 1, 2 ** 20 + 1):
+        with pytest.raises(ValueError, match=str(2 ** 25)):
             colearn_attention(rows(h), rows(h), rows(h))
-        with pytest.raises(ValueError, match="8388608"):
+        with pytest.raises(ValueError, match=str(2 ** 25)):
             colearn_attention(rows(h), rows(1), rows(1))
-    x = torch.randn(1, 3, 2 ** 16, 128, device="cuda").to(torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 40, 128])
+def test_the_largest_tokens(d):
+    """A whole tile of tokens of 2^25 elements, or just below: the last heads'
+    rows lie 2^32 bytes from the first."""
+    h = 2 ** 25 // d
+    g = torch.Generator("cuda").manual_seed(0)
+    x = torch.empty(1, 64, h, d, dtype=torch.bfloat16, device="cuda")
+    x.normal_(generator=g)
     out = colearn_attention(x, x, x)
-    for part in (slice(0, 4), slice(2 ** 16 - 4, 2 ** 16)):
+    for part in (slice(0, 4), slice(h // 2, h // 2 + 4), slice(h - 4, h)):
         few = x[:, :, part].contiguous()
         assert torch.equal(out[:, :, part], colearn_attention(few, few, few))
 
